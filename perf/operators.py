@@ -138,7 +138,7 @@ def _quantize(x, rows):
     m, k = x.shape
     blocks = _blocked(x, rows)
     a = blocks.abs().amax((1, 3)).clamp_min(FLOOR)
-    code = (blocks * (TOP / a)[:, None, :, None]).clamp(-TOP, TOP).to(E4M3)
+    code = (blocks * torch.full_like(a, TOP).div(a)[:, None, :, None]).clamp(-TOP, TOP).to(E4M3)
     return code.view(-1, blocks.shape[2] * 128)[:m, :k], a / TOP
 
 
