@@ -338,6 +338,66 @@ int lcg_swiglu(const void* z, int64_t M, int64_t I, int64_t ldz, void* s, int64_
  * the layer in config form `x + mlp(x)`). n % 8 == 0. */
 int lcg_add(const void* a, const void* b, void* out, int64_t n, void* stream);
 
+/* ---- 8-bit products with a scale for each block of 128 --------------------
+ * No counterpart in the reference, whose path is bf16 throughout.  Operands are e4m3 codes (one
+ * byte each, row-major, K-major like every operand here) with one fp32 scale per block of 128
+ * consecutive values of a row: value = code * scale.  An activation has its own scales in every
+ * row, a weight shares each scale among 128 rows.  A scale is found at
+ * scale[row_block * row_stride + k_block * block_stride], so either order of the two works; the
+ * producers below are fastest with row_stride = 1.  K need not be a multiple of 128: the last
+ * block is then shorter.  Codes have a pitch of a multiple of 16 bytes and a 16-byte aligned base.
+ *
+ * A producer scales one block by a = max(max |x|, 2^-100): scale = a / 448, code =
+ * e4m3(x * (448 / a)), with correctly rounded fp32 arithmetic and one rounding to e4m3 (nearest
+ * even, saturating).  A block that holds an infinity or a NaN decodes to NaN throughout.  The columns
+ * from K to the next multiple of 16 receive zero codes. */
+
+/* Codes and scales of a bf16 matrix x (M, K) with leading dimension ldx.  block_rows = 1: a scale
+ * per row and block (activations); 128: a scale per 128 x 128 tile (weights).  Any M, K >= 1; rows
+ * that are not 16-byte aligned are read value by value. */
+int lcg_quantize_fp8(const void* x, int64_t M, int64_t K, int64_t ldx, int block_rows, void* q,
+                     int64_t ldq, float* scale, int64_t scale_row_stride,
+                     int64_t scale_block_stride, void* stream);
+
+/* lcg_add_rmsnorm with an 8-bit result: h = bf16(delta + residual) -> residual_out (may alias
+ * residual), y = h * rsqrt(mean(h^2) + eps) * (norm_weight + 1), quantised by rows from its fp32
+ * value (it is never rounded to bf16).  delta may be NULL: h is the residual, residual_out is
+ * neither needed nor written.  Contiguous (M, K), K % 8 == 0, K <= 24576. */
+int lcg_add_rmsnorm_fp8(const void* delta, const void* residual, const void* norm_weight,
+                        int64_t M, int64_t K, float eps, void* residual_out, void* q, int64_t ldq,
+                        float* scale, int64_t scale_row_stride, int64_t scale_block_stride,
+                        void* stream);
+
+/* lcg_swiglu with an 8-bit result: silu(gate) * up quantised by rows from its fp32 value.  z is
+ * (M, 2*I) with ldz; I % 8 == 0. */
+int lcg_swiglu_fp8(const void* z, int64_t M, int64_t I, int64_t ldz, void* q, int64_t ldq,
+                   float* scale, int64_t scale_row_stride, int64_t scale_block_stride,
+                   void* stream);
+
+/* C = bf16(sum over blocks t of a_scale[m, t] * b_scale[n / 128, t] * (a . b over block t)), block
+ * sums and scaled sum in fp32.  a (M, K) and b (N, K) codes, scales of `block_rows` 1 and 128; c
+ * (M, N) bf16, 16-byte aligned, ldc % 8 == 0.  Any M, N, K >= 1, one token included. */
+int lcg_gemm_fp8(const void* a, int64_t lda, const float* a_scale, int64_t a_scale_row_stride,
+                 int64_t a_scale_block_stride, const void* b, int64_t ldb, const float* b_scale,
+                 int64_t b_scale_row_stride, int64_t b_scale_block_stride, void* c, int64_t ldc,
+                 int64_t M, int64_t N, int64_t K, int32_t* status, void* stream);
+
+/* ---- log probabilities ----------------------------------------------------
+ * For each row of logits (M, V), leading dimension ld, of type bf16, fp16 or fp32:
+ *   logprob = x[token] - ln(sum e^x)       entropy = -sum p ln p
+ * and the `top` (0..32, at most V) largest values with their log probabilities, largest first,
+ * equal values by rising id.  tokens: M ids of token_bytes (4 or 8) bytes each.  A masked value
+ * (-inf) has probability 0 and log probability -inf.  A row that is all -inf, or that holds +inf or
+ * a NaN, has no distribution: its numbers are NaN (its ids are still distinct and in range; a NaN
+ * ranks with -inf).  An id outside [0, V) gives NaN for that row's logprob and is not read.  The
+ * agreement measures of the reference work on these numbers (lcgemm/bench/prefill.py:180-197). */
+#define LCG_DTYPE_BF16 0
+#define LCG_DTYPE_FP16 1
+#define LCG_DTYPE_FP32 2
+int lcg_token_logprobs(const void* logits, int dtype, int64_t M, int64_t V, int64_t ld,
+                       const void* tokens, int token_bytes, int top, float* logprob,
+                       float* entropy, float* top_logprobs, int64_t* top_ids, void* stream);
+
 /* ---- introspection ------------------------------------------------------- */
 
 /* Kernel launches issued by this library in this process (for the bench's

@@ -17,12 +17,14 @@ INCLUDE = _PKG.parent.parent / "include"
 LIB_DIR = _PKG / "_lib"
 # LCGEMM_B200_LIB points the loader at another build of the same sources (an A/B comparison).
 LIB_PATH = Path(os.environ.get("LCGEMM_B200_LIB") or LIB_DIR / "liblcgemm_b200.so")
-SOURCES = ("lcg_scheme.cu", "lcg_simt.cu", "lcg_gemm.cu", "lcg_static.cu", "lcg_peer.cu")
+SOURCES = ("lcg_scheme.cu", "lcg_simt.cu", "lcg_gemm.cu", "lcg_static.cu", "lcg_peer.cu",
+           "lcg_fp8.cu", "lcg_fp8_gemm.cu", "lcg_logprobs.cu")
 
 OK = 0
 ERR_BAD_ARG, ERR_UNSUPPORTED_SHAPE, ERR_MISALIGNED, ERR_SCHEME, ERR_CUDA, ERR_DEVICE_TIMEOUT = (
     -1, -2, -3, -4, -5, -6)
 SCHEDULE_ALL_RANKS, SCHEDULE_RANK_SPLIT, SCHEDULE_HYBRID = 0, 1, 2
+DTYPE_BF16, DTYPE_FP16, DTYPE_FP32 = 0, 1, 2
 
 _c = ctypes
 _vp, _i64, _i32, _f32 = _c.c_void_p, _c.c_int64, _c.c_int, _c.c_float
@@ -67,6 +69,12 @@ SIGNATURES = {
     "lcg_add_rmsnorm": (_i32, [_vp, _vp, _vp, _i64, _i64, _f32, _vp, _vp, _vp]),
     "lcg_swiglu": (_i32, [_vp, _i64, _i64, _i64, _vp, _i64, _vp]),
     "lcg_add": (_i32, [_vp, _vp, _vp, _i64, _vp]),
+    "lcg_quantize_fp8": (_i32, [_vp, _i64, _i64, _i64, _i32, _vp, _i64, _vp, _i64, _i64, _vp]),
+    "lcg_add_rmsnorm_fp8": (_i32, [_vp, _vp, _vp, _i64, _i64, _f32, _vp, _vp, _i64, _vp, _i64, _i64, _vp]),
+    "lcg_swiglu_fp8": (_i32, [_vp, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _vp]),
+    "lcg_gemm_fp8": (_i32, [_vp, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _i64,
+                            _vp, _vp]),
+    "lcg_token_logprobs": (_i32, [_vp, _i32, _i64, _i64, _i64, _vp, _i32, _i32, _vp, _vp, _vp, _vp, _vp]),
     "lcg_launch_count": (_i64, []),
     "lcg_describe_gemm": (_i32, [_i64, _i64, _i64, _i32, _i32, _i32, _c.c_char_p, _i32]),
 }

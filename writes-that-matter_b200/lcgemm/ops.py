@@ -2,11 +2,14 @@
 
 Every function here launches CUDA work on the current torch stream through
 ``include/lcgemm_b200.h`` and never synchronises.  Tensors must be bf16 CUDA
-tensors; there is no CPU implementation behind these calls.
+tensors (the 8-bit products take e4m3 codes with fp32 scales, the log probabilities
+also fp16 and fp32 logits); there is no CPU implementation behind these calls.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
+from typing import NamedTuple
 
 import torch
 
@@ -14,6 +17,8 @@ from . import _native as nat
 from ._native import NativeScheme, check, lib, ptr, stream_ptr
 
 BF16 = torch.bfloat16
+E4M3 = torch.float8_e4m3fn
+FP8_BLOCK = 128                  # values of a row under one scale
 
 _STATUS: dict = {}
 
@@ -448,3 +453,181 @@ def add(a: torch.Tensor, b: torch.Tensor, out: torch.Tensor | None = None) -> to
         out = torch.empty_like(a)
     check(lib().lcg_add(ptr(a), ptr(b), ptr(out), a.numel(), stream_ptr()))
     return out
+
+
+# ------------------------------------------- 8-bit operands, a scale per 128
+def _on(t: torch.Tensor, *others):
+    """Context in which ``t``'s device is current; every tensor of a call lives there."""
+    for o in others:
+        if o is not None and o.device != t.device:
+            raise ValueError(f"all tensors of a call must be on one device, got {t.device} and {o.device}")
+    if t.device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(t.device)
+
+
+def _codes(m: int, k: int, device):
+    """An (m, k) view of codes whose row pitch is a multiple of 16 bytes."""
+    return torch.empty((m, (k + 15) // 16 * 16), dtype=E4M3, device=device)[:, :k]
+
+
+def _row_scales(m: int, k: int, device):
+    """(m, blocks) scales with the rows contiguous: the order the product reads fastest."""
+    return torch.empty((-(-k // FP8_BLOCK), m), dtype=torch.float32, device=device).t()
+
+
+def quantize_fp8(x: torch.Tensor, block_rows: int = 1):
+    """``(codes, scales)`` of a bf16 matrix ``(M, K)``: e4m3 codes ``(M, K)`` and one fp32 scale per
+    block, ``code * scale`` being the value.  ``block_rows=1`` scales 128 values of a row at a time,
+    scales ``(M, ceil(K / 128))`` (activations); ``block_rows=128`` scales 128 x 128 tiles, scales
+    ``(ceil(M / 128), ceil(K / 128))`` (weights).  ``scale = a / 448`` with ``a = max(max |x|, 2^-100)``; a
+    block that holds an infinity or a NaN decodes to NaN."""
+    _need(x, "x")
+    if x.dim() != 2:
+        raise ValueError(f"x must be a matrix, got {tuple(x.shape)}")
+    if block_rows not in (1, FP8_BLOCK):
+        raise ValueError(f"block_rows must be 1 or {FP8_BLOCK}, got {block_rows}")
+    m, k = x.shape
+    if k < 1:
+        raise ValueError("x has no columns")
+    with _on(x):
+        q = _codes(m, k, x.device)
+        if block_rows == 1:
+            scale = _row_scales(m, k, x.device)
+        else:
+            scale = torch.empty((-(-m // FP8_BLOCK), -(-k // FP8_BLOCK)), dtype=torch.float32, device=x.device)
+        if m > 0:
+            check(lib().lcg_quantize_fp8(ptr(x), m, k, x.stride(0), block_rows, ptr(q), q.stride(0), ptr(scale),
+                                         scale.stride(0), scale.stride(1), stream_ptr()))
+    return q, scale
+
+
+def add_rmsnorm_fp8(delta, residual, norm_weight, eps: float, residual_out=None):
+    """:func:`add_rmsnorm` with an 8-bit result: ``(codes, scales, delta + residual)``, the norm
+    quantised by rows from its fp32 value.  Without a ``delta`` the third value is ``residual`` itself
+    and nothing is stored for it.  ``residual_out`` may be ``residual``."""
+    tensors = [(residual, "residual"), (norm_weight, "norm weight")]
+    if delta is not None:
+        tensors.append((delta, "delta"))
+        if residual_out is not None:
+            tensors.append((residual_out, "residual_out"))
+    for t, what in tensors:
+        _need(t, what)
+    if residual.dim() != 2:
+        raise ValueError(f"residual must be a matrix, got {tuple(residual.shape)}")
+    m, k = residual.shape
+    for t, what in tensors:
+        want = (k,) if t is norm_weight else (m, k)
+        if tuple(t.shape) != want or not t.is_contiguous():
+            raise ValueError(f"{what} must be a contiguous {want} tensor")
+    with _on(residual, norm_weight, delta, residual_out):
+        if delta is None:
+            residual_out = None
+        elif residual_out is None:
+            residual_out = torch.empty_like(residual)
+        q, scale = _codes(m, k, residual.device), _row_scales(m, k, residual.device)
+        if m > 0:
+            check(lib().lcg_add_rmsnorm_fp8(None if delta is None else ptr(delta), ptr(residual), ptr(norm_weight), m, k,
+                                            float(eps), None if delta is None else ptr(residual_out), ptr(q),
+                                            q.stride(0), ptr(scale), scale.stride(0), scale.stride(1), stream_ptr()))
+    return q, scale, residual if delta is None else residual_out
+
+
+def swiglu_fp8(z: torch.Tensor):
+    """``(codes, scales)`` of ``silu(z[:, :I]) * z[:, I:]``, quantised by rows from its fp32 value."""
+    _need(z, "z")
+    if z.dim() != 2 or z.shape[1] % 2 != 0:
+        raise ValueError(f"z must be an (M, 2 * I) matrix, got {tuple(z.shape)}")
+    m, inter = z.shape[0], z.shape[1] // 2
+    with _on(z):
+        q, scale = _codes(m, inter, z.device), _row_scales(m, inter, z.device)
+        if m > 0:
+            check(lib().lcg_swiglu_fp8(ptr(z), m, inter, z.stride(0), ptr(q), q.stride(0), ptr(scale),
+                                       scale.stride(0), scale.stride(1), stream_ptr()))
+    return q, scale
+
+
+def gemm_fp8(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor,
+             out: torch.Tensor | None = None) -> torch.Tensor:
+    """``a @ b.T`` in bf16 from e4m3 codes ``a (M, K)`` and ``b (N, K)`` with one fp32 scale per block of
+    128: ``a_scale (M, ceil(K / 128))``, ``b_scale (ceil(N / 128), ceil(K / 128))``, of any strides (the
+    quantisers' are the fastest).  Codes have unit stride along K and a row pitch of a multiple of 16
+    bytes, as the quantisers return them.  Each block's sum and the scaled sum are fp32."""
+    for t, what in ((a, "a"), (b, "b"), (a_scale, "a_scale"), (b_scale, "b_scale")):
+        if not isinstance(t, torch.Tensor) or not t.is_cuda:
+            raise RuntimeError(
+                f"{what} must be a CUDA tensor: lcgemm_b200 has no CPU implementation of this path")
+        if t.dim() != 2:
+            raise ValueError(f"{what} must be a matrix, got {tuple(t.shape)}")
+    if a.dtype != E4M3 or b.dtype != E4M3:
+        raise ValueError(f"a and b must be float8_e4m3fn, got {a.dtype} and {b.dtype}")
+    if a_scale.dtype != torch.float32 or b_scale.dtype != torch.float32:
+        raise ValueError(f"scales must be float32, got {a_scale.dtype} and {b_scale.dtype}")
+    (m, k), (n, kb) = a.shape, b.shape
+    if kb != k:
+        raise ValueError(f"inner dimensions differ: {k} vs {kb}")
+    if k < 1 or n < 1:
+        raise ValueError(f"empty product: N={n}, K={k}")
+    if (a.stride(1) != 1 or b.stride(1) != 1) and k > 1:
+        raise ValueError("codes must be row-major (unit stride along their last dimension)")
+    blocks = -(-k // FP8_BLOCK)
+    if tuple(a_scale.shape) != (m, blocks) or tuple(b_scale.shape) != (-(-n // FP8_BLOCK), blocks):
+        raise ValueError(f"scales must be {(m, blocks)} and {(-(-n // FP8_BLOCK), blocks)}, got "
+                         f"{tuple(a_scale.shape)} and {tuple(b_scale.shape)}")
+    if out is not None:
+        _need(out, "out")
+        if tuple(out.shape) != (m, n):
+            raise ValueError(f"out must be ({m}, {n}), got {tuple(out.shape)}")
+    with _on(a, b, a_scale, b_scale, out):
+        if out is None:
+            out = _padded_out(m, n, a.device)
+        if m > 0:
+            check(lib().lcg_gemm_fp8(ptr(a), a.stride(0), ptr(a_scale), a_scale.stride(0), a_scale.stride(1),
+                                     ptr(b), b.stride(0), ptr(b_scale), b_scale.stride(0), b_scale.stride(1),
+                                     ptr(out), out.stride(0), m, n, k, ptr(status_word(a.device)), stream_ptr()))
+    return out
+
+
+# ---------------------------------------------------------- log probabilities
+class TokenLogprobs(NamedTuple):
+    logprob: torch.Tensor          # (M,) fp32
+    entropy: torch.Tensor          # (M,) fp32, in nats
+    top_logprobs: torch.Tensor     # (M, top) fp32, largest first
+    top_ids: torch.Tensor          # (M, top) int64, equal values by rising id
+
+
+MAX_TOP = 32
+_LOGIT_TYPES = {BF16: nat.DTYPE_BF16, torch.float16: nat.DTYPE_FP16, torch.float32: nat.DTYPE_FP32}
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> TokenLogprobs:
+    """Log probability of ``tokens[i]`` under ``softmax(logits[i])``, each row's entropy, and its ``top``
+    (0 to 32) most likely tokens, in one pass over ``logits (M, V)`` (bf16, fp16 or fp32, unit stride along
+    V).  ``-inf`` masks a token.  A row that is all ``-inf``, or holds ``+inf`` or a NaN, gives NaN; an id
+    outside ``[0, V)`` gives a NaN log probability for its row."""
+    for t, what in ((logits, "logits"), (tokens, "tokens")):
+        if not isinstance(t, torch.Tensor) or not t.is_cuda:
+            raise RuntimeError(
+                f"{what} must be a CUDA tensor: lcgemm_b200 has no CPU implementation of this path")
+    kind = _LOGIT_TYPES.get(logits.dtype)
+    if kind is None:
+        raise ValueError(f"logits must be bfloat16, float16 or float32, got {logits.dtype}")
+    if logits.dim() != 2 or (logits.stride(1) != 1 and logits.shape[1] > 1):
+        raise ValueError(f"logits must be a row-major (M, V) matrix, got {tuple(logits.shape)}")
+    m, v = logits.shape
+    if tokens.dtype not in (torch.int64, torch.int32) or tuple(tokens.shape) != (m,):
+        raise ValueError(f"tokens must be ({m},) of int64 or int32, got {tuple(tokens.shape)} of {tokens.dtype}")
+    if not 0 <= top <= min(MAX_TOP, v):
+        raise ValueError(f"top must be between 0 and {min(MAX_TOP, v)}, got {top}")
+    if v < 1:
+        raise ValueError("logits have no columns")
+    with _on(logits, tokens):
+        tokens = tokens.contiguous()
+        dev = logits.device
+        logprob, entropy = torch.empty((2, m), dtype=torch.float32, device=dev).unbind(0)
+        top_lp = torch.empty((m, top), dtype=torch.float32, device=dev)
+        top_ids = torch.empty((m, top), dtype=torch.int64, device=dev)
+        if m > 0:
+            check(lib().lcg_token_logprobs(ptr(logits), kind, m, v, logits.stride(0), ptr(tokens), tokens.element_size(),
+                                           top, ptr(logprob), ptr(entropy), ptr(top_lp), ptr(top_ids), stream_ptr()))
+    return TokenLogprobs(logprob, entropy, top_lp, top_ids)
