@@ -23,6 +23,15 @@ void count_launch(int n = 1);
       return ::lcg::fail(LCG_ERR_CUDA, "%s: %s", #expr, cudaGetErrorString(_e)); \
   } while (0)
 
+// ---- host helpers of the tcgen05 kernels (lcg_gemm.cu) ---------------------
+// Row-major (outer x inner) matrix of leading dimension `ld` elements, boxes of box_outer rows x 128
+// bytes with the 128-byte swizzle, zeros outside the matrix.
+int make_tensor_map(CUtensorMap* map, CUtensorMapDataType type, int elt_bytes, const void* base,
+                    int64_t inner, int64_t outer, int64_t ld, int box_outer, const char* what);
+int sm_count();
+// Tile rows kept open at once: the divisor-free version of "minimise a + groups / a".
+int pick_group_m(int tiles_m, int groups);
+
 // ---- what the kernel needs to know about one accumulator step -------------
 struct EpiDest {
   int8_t bi, bj;     // destination C block

@@ -1048,23 +1048,24 @@ EncodeFn encode_fn() {
   return fn;
 }
 
-// bf16 row-major (outer x inner) matrix, 128-byte swizzled boxes of box_outer x 64.
-int make_map(CUtensorMap* map, const void* base, int64_t inner, int64_t outer, int64_t ld,
-             int box_outer, const char* what) {
+}  // namespace
+
+int make_tensor_map(CUtensorMap* map, CUtensorMapDataType type, int elt_bytes, const void* base,
+                    int64_t inner, int64_t outer, int64_t ld, int box_outer, const char* what) {
   EncodeFn fn = encode_fn();
   if (fn == nullptr) return fail(LCG_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
   if ((reinterpret_cast<uintptr_t>(base) & 15u) != 0)
     return fail(LCG_ERR_MISALIGNED, "%s: base address must be 16-byte aligned", what);
-  if (ld % 8 != 0)
-    return fail(LCG_ERR_MISALIGNED, "%s: leading dimension %lld must be a multiple of 8 elements", what,
-                (long long)ld);
+  if (ld * elt_bytes % 16 != 0)
+    return fail(LCG_ERR_MISALIGNED, "%s: leading dimension %lld must be a multiple of %d elements", what,
+                (long long)ld, 16 / elt_bytes);
   if (inner < 1 || outer < 1) return fail(LCG_ERR_UNSUPPORTED_SHAPE, "%s: empty extent", what);
   const cuuint64_t dims[2] = {static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(outer)};
-  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld) * 2};
-  const cuuint32_t box[2] = {static_cast<cuuint32_t>(kBK), static_cast<cuuint32_t>(box_outer)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld) * elt_bytes};
+  const cuuint32_t box[2] = {static_cast<cuuint32_t>(128 / elt_bytes), static_cast<cuuint32_t>(box_outer)};
   const cuuint32_t estr[2] = {1, 1};
   const CUresult r =
-      fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, estr,
+      fn(map, type, 2, const_cast<void*>(base), dims, strides, box, estr,
          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS)
@@ -1083,7 +1084,6 @@ int sm_count() {
   return sms;
 }
 
-// Tile rows kept open at once: the divisor-free version of "minimise a + groups / a".
 int pick_group_m(int tiles_m, int groups) {
   int best = 1;
   double best_cost = 1e30;
@@ -1096,6 +1096,14 @@ int pick_group_m(int tiles_m, int groups) {
     }
   }
   return best;
+}
+
+namespace {
+
+// bf16 row-major (outer x inner) matrix, 128-byte swizzled boxes of box_outer x 64.
+int make_map(CUtensorMap* map, const void* base, int64_t inner, int64_t outer, int64_t ld,
+             int box_outer, const char* what) {
+  return make_tensor_map(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base, inner, outer, ld, box_outer, what);
 }
 
 template <int kCtaGroup, int kMode, unsigned long long kPlaneCode = 0>

@@ -102,7 +102,7 @@ struct WaitCtl {
   uint64_t limit_ns = kWaitLimitNs;
 };
 
-__device__ __noinline__ void mbar_wait_slow(uint32_t bar, uint32_t parity, const WaitCtl& ctl,
+static __device__ __noinline__ void mbar_wait_slow(uint32_t bar, uint32_t parity, const WaitCtl& ctl,
                                             int code) {
   if (*ctl.abort_flag) return;
   const uint64_t t0 = globaltimer_ns();
@@ -125,6 +125,21 @@ __device__ __forceinline__ void mbar_wait(uint32_t bar, uint32_t parity, const W
   mbar_wait_slow(bar, parity, ctl, code);
 }
 
+// The same without a call: for warps whose registers are full of accumulators, which a call's
+// register convention would move about.
+__device__ __forceinline__ void mbar_wait_inline(uint32_t bar, uint32_t parity, const WaitCtl& ctl, int code) {
+  if (mbar_try_wait(bar, parity)) return;
+  const uint64_t t0 = globaltimer_ns();
+  while (!mbar_try_wait(bar, parity)) {
+    if (*ctl.abort_flag) return;
+    if (globaltimer_ns() - t0 > ctl.limit_ns) {
+      *ctl.abort_flag = 1u;
+      if (ctl.status != nullptr) atomicCAS(ctl.status, 0, code);
+      return;
+    }
+  }
+}
+
 // Bounded wait on a monotonically increasing shared-memory counter.
 __device__ __forceinline__ uint32_t ld_acquire_shared(uint32_t addr) {
   uint32_t v;
@@ -135,7 +150,7 @@ __device__ __forceinline__ void st_release_shared(uint32_t addr, uint32_t v) {
   asm volatile("st.release.cta.shared::cta.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
 }
 
-__device__ __noinline__ void counter_wait(uint32_t addr, uint32_t at_least, const WaitCtl& ctl,
+static __device__ __noinline__ void counter_wait(uint32_t addr, uint32_t at_least, const WaitCtl& ctl,
                                           int code) {
   if (ld_acquire_shared(addr) >= at_least) return;
   if (*ctl.abort_flag) return;
@@ -161,7 +176,7 @@ __device__ __forceinline__ uint32_t ld_acquire_gpu(const uint32_t* p) {
   asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
   return v;
 }
-__device__ __noinline__ void global_counter_wait(const uint32_t* ctr, uint32_t at_least,
+static __device__ __noinline__ void global_counter_wait(const uint32_t* ctr, uint32_t at_least,
                                                  const WaitCtl& ctl, int code) {
   if (ld_acquire_gpu(ctr) >= at_least) return;
   if (*ctl.abort_flag) return;
@@ -316,6 +331,33 @@ __device__ __forceinline__ void umma_bf16(uint32_t tmem_d, uint64_t desc_a, uint
   }
 }
 
+// The same for 8-bit operands (e4m3), K = 32 per instruction.
+template <int kCtaGroup>
+__device__ __forceinline__ void umma_fp8(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b,
+                                         uint32_t idesc, uint32_t accumulate) {
+  if constexpr (kCtaGroup == 1) {
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t"
+        "}\n"
+        :
+        : "r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+        : "memory");
+  } else {
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t"
+        "}\n"
+        :
+        : "r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+        : "memory");
+  }
+}
+
 // Make `bar` (same shared-memory offset in every CTA of the group) complete one
 // arrival when all tcgen05 operations issued so far by this thread are done.
 template <int kCtaGroup>
@@ -349,6 +391,27 @@ __device__ __forceinline__ void tmem_ld_32x32(uint32_t taddr, uint32_t (&r)[32])
       : "memory");
 }
 
+// The same, 16 columns.
+__device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+
+// Wait for the loads in flight, naming the registers of one of them: what uses them stays behind it.
+__device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+               :
+               : "memory");
+}
+
 __device__ __forceinline__ void tmem_ld_wait() {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
@@ -378,6 +441,26 @@ __device__ __forceinline__ uint64_t make_kmajor_sw128_desc(uint32_t smem_addr) {
 __host__ __device__ constexpr uint32_t make_idesc_bf16(int m, int n) {
   return (1u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(n >> 3) << 17) |
          (static_cast<uint32_t>(m >> 4) << 24);
+}
+
+// Instruction descriptor, kind::f8f6f4: D fp32, A and B e4m3 (format 0), both K-major.
+__host__ __device__ constexpr uint32_t make_idesc_e4m3(int m, int n) {
+  return (1u << 4) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
+}
+
+// Two fp32 in one register pair: d = a * b + c for both halves in one instruction.
+__device__ __forceinline__ uint64_t pack_f32x2(uint32_t lo, uint32_t hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
+  return r;
+}
+__device__ __forceinline__ void unpack_f32x2(uint64_t v, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
 }
 
 }  // namespace lcg
