@@ -243,7 +243,7 @@ k_gemm_fp8(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CU
               if (c + 1 == kChunks) {       // everything is in registers: the stage is free
                 tcgen05_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive_cluster(acc_empty_leader + 8u * as);
+                if (lane == 0) mbar_arrive_cluster_relaxed(acc_empty_leader + 8u * as);
               }
 #pragma unroll
               for (int j = 0; j < 8; ++j)
