@@ -52,17 +52,29 @@ __device__ __forceinline__ void regs_dec() {
 constexpr int kCodeProducer = 101, kCodeMmaAcc = 102, kCodeMmaFull = 103, kCodeEpilogue = 104;
 
 // ================================================================ many rows
-// 12 warps: 0 TMA producer, 1 MMA issuer, 2 and 3 idle (a register split goes by warpgroups),
-// 4-7 and 8-11 read-back: every warp one TMEM lane quarter, each warpgroup half of the columns.
+// A pair multiplies 256 rows of a by kBN rows of b, 128 columns of the accumulator at a time: TMEM
+// holds four stages of 128 columns, so that a block's sums stay there while they are read back and
+// the next ones are being formed.  (Two stages of 256 columns would take half as many instructions, but
+// a stage is then handed back so late that the tensor cores wait for it.)
+//
+// 12 warps: 0 TMA producer, 1 MMA issuer, 2 and 3 scales, 4-7 and 8-11 read-back: every warp one
+// TMEM lane quarter, each warpgroup half of a stage's columns.  Columns [0, 64) of stage h of a
+// tile come from rows 64 h .. of the b tile in CTA 0 and columns [64, 128) from CTA 1's, so
+// warpgroup w owns columns [w * kBN / 2, (w + 1) * kBN / 2) of the tile.
 template <int kBN>
 struct Many {
-  static constexpr int kAcc = 512 / kBN;                    // TMEM stages
+  static constexpr int kAccCols = 128;
+  static constexpr int kAcc = 512 / kAccCols;               // TMEM stages
+  static constexpr int kParts = kBN / kAccCols;             // stages a K block fills
   static constexpr int kBRows = kBN / 2;                    // rows of b each CTA of the pair loads
   static constexpr int kStageBytes = kOperandBytes + kBRows * kBlock;
-  static constexpr int kStages = kBN == 256 ? 6 : 8;
+  static constexpr int kStages = kBN == 256 ? 5 : 7;
   static constexpr int kCols = kBN / 2;                     // columns per read-back warpgroup
   static constexpr int kStoreBytes = 32 * 128;              // a warp's staged 32 x 64 bf16
-  static constexpr int kSmemBytes = kStages * kStageBytes + 8 * kStoreBytes + 256 + 1024;
+  static constexpr int kGroup = 4;                          // K blocks whose scales travel together
+  static constexpr int kSlots = 4;
+  static constexpr int kSlotFloats = kGroup * 2 * kTileRows;
+  static constexpr int kSmemBytes = kStages * kStageBytes + 8 * kStoreBytes + kSlots * kSlotFloats * 4 + 256 + 1024;
 };
 constexpr int kManyThreads = 384;
 
@@ -83,16 +95,22 @@ k_gemm_fp8(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CU
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
   const uint32_t store_base = base + T::kStages * T::kStageBytes;
-  const uint32_t bar_base = store_base + 8 * T::kStoreBytes;
+  const uint32_t scale_base = store_base + 8 * T::kStoreBytes;
+  float* scales = reinterpret_cast<float*>(smem_raw + (scale_base - raw));
+  const uint32_t bar_base = scale_base + T::kSlots * T::kSlotFloats * 4;
   auto full_bar = [&](uint32_t s) { return bar_base + 8u * s; };
   auto empty_bar = [&](uint32_t s) { return bar_base + 8u * (T::kStages + s); };
   auto acc_full_bar = [&](uint32_t s) { return bar_base + 8u * (2 * T::kStages + s); };
   auto acc_empty_bar = [&](uint32_t s) { return bar_base + 8u * (2 * T::kStages + T::kAcc + s); };
-  const uint32_t misc = bar_base + 8u * (2 * T::kStages + 2 * T::kAcc);
+  auto scale_full_bar = [&](uint32_t s) { return bar_base + 8u * (2 * T::kStages + 2 * T::kAcc + s); };
+  auto scale_empty_bar = [&](uint32_t s) { return bar_base + 8u * (2 * T::kStages + 2 * T::kAcc + T::kSlots + s); };
+  const uint32_t misc = bar_base + 8u * (2 * T::kStages + 2 * T::kAcc + 2 * T::kSlots);
+  static_assert(8 * (2 * T::kStages + 2 * T::kAcc + 2 * T::kSlots) + 8 <= 256, "barrier area");
   volatile uint32_t* misc_gen = reinterpret_cast<volatile uint32_t*>(smem_raw + (misc - raw));
   // misc_gen[0] = TMEM base, [1] = abort flag
 
-  const int warp = threadIdx.x >> 5;
+  // warp-uniform by construction, so that the single-thread roles keep their state in uniform registers
+  const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
   const int lane = threadIdx.x & 31;
   const uint32_t cta_rank = cluster_ctarank();
   const bool leader = cta_rank == 0;
@@ -109,6 +127,10 @@ k_gemm_fp8(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CU
       mbar_init(acc_full_bar(s), 1);
       mbar_init(acc_empty_bar(s), 16);     // the read-back warps of both CTAs
     }
+    for (uint32_t s = 0; s < T::kSlots; ++s) {
+      mbar_init(scale_full_bar(s), 2);     // both scale warps
+      mbar_init(scale_empty_bar(s), 8);    // the read-back warps of this CTA
+    }
     misc_gen[1] = 0u;
     fence_mbar_init();
     prefetch_tensormap(&tma_a);
@@ -124,7 +146,7 @@ k_gemm_fp8(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CU
   cluster_arrive();
   cluster_wait();
   tcgen05_fence_after();
-  const uint32_t tmem_base = misc_gen[0];
+  const uint32_t tmem_base = __shfl_sync(0xffffffffu, misc_gen[0], 0);
 
   // Bands of group_m tile rows, tile row fastest inside a band (lcg_gemm.cu: tile_coord).
   auto tile_at = [&](int t, int& tm, int& tn) {
@@ -137,8 +159,8 @@ k_gemm_fp8(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CU
   };
 
   if (warp < 4) {
-    regs_dec<56>();
-    if (warp == 0 && lane == 0) {
+    regs_dec<40>();
+    if (warp == 0) {
       // ---------------------------------------------------------- TMA producer
       uint32_t stage = 0, wait_parity = 1;
       const uint32_t full_leader = mapa_shared(full_bar(0), 0);
@@ -149,114 +171,176 @@ k_gemm_fp8(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CU
         const int b_row = tn * kBN + static_cast<int>(cta_rank) * T::kBRows;
         for (int kb = 0; kb < p.k_blocks; ++kb) {
           mbar_wait_inline(empty_bar(stage), wait_parity, ctl, kCodeProducer);
-          if (leader) mbar_arrive_expect_tx(full_bar(stage), 2 * T::kStageBytes);
-          const uint32_t sa = base + stage * T::kStageBytes;
-          const uint32_t bar = full_leader + 8u * stage;
-          tma_load_2d_pair(sa, &tma_a, bar, kb * kBlock, a_row);
-          tma_load_2d_pair(sa + kOperandBytes, &tma_b, bar, kb * kBlock, b_row);
+          if (elect_one()) {
+            if (leader) mbar_arrive_expect_tx(full_bar(stage), 2 * T::kStageBytes);
+            const uint32_t sa = base + stage * T::kStageBytes;
+            const uint32_t bar = full_leader + 8u * stage;
+            tma_load_2d_pair(sa, &tma_a, bar, kb * kBlock, a_row);
+            tma_load_2d_pair(sa + kOperandBytes, &tma_b, bar, kb * kBlock, b_row);
+          }
+          __syncwarp();
           if (++stage == T::kStages) {
             stage = 0;
             wait_parity ^= 1u;
           }
         }
       }
-    } else if (warp == 1 && lane == 0 && leader) {
+    } else if (warp == 1) {
       // ------------------------------------------------------------ MMA issuer
-      constexpr uint32_t idesc = make_idesc_e4m3(2 * kTileRows, kBN);
-      const uint64_t adesc0 = make_kmajor_sw128_desc(base);
-      const uint64_t bdesc0 = make_kmajor_sw128_desc(base + kOperandBytes);
-      uint32_t stage = 0, parity = 0, as = 0, acc_parity = 1;
-      for (int t = pair; t < p.num_tiles; t += num_pairs) {
-        for (int kb = 0; kb < p.k_blocks; ++kb) {
-          mbar_wait_inline(acc_empty_bar(as), acc_parity, ctl, kCodeMmaAcc);
-          mbar_wait_inline(full_bar(stage), parity, ctl, kCodeMmaFull);
-          tcgen05_fence_after();
-          const uint64_t soff = static_cast<uint64_t>(stage * (T::kStageBytes >> 4));
+      // The whole warp walks the loop and one lane issues: descriptors and addresses then live in
+      // uniform registers.  With one lane in the loop every instruction first moved its operands
+      // there, 75 cycles for each MMA, more than the MMA takes.
+      if (leader) {
+        constexpr uint32_t idesc = make_idesc_e4m3(2 * kTileRows, T::kAccCols);
+        const uint64_t adesc0 = make_kmajor_sw128_desc(base);
+        const uint64_t bdesc0 = make_kmajor_sw128_desc(base + kOperandBytes);
+        uint32_t stage = 0, parity = 0, as = 0, acc_parity = 1;
+        for (int t = pair; t < p.num_tiles; t += num_pairs) {
+          for (int kb = 0; kb < p.k_blocks; ++kb) {
+            const uint64_t soff = static_cast<uint64_t>(stage * (T::kStageBytes >> 4));
 #pragma unroll
-          for (int k = 0; k < kBlock / kSliceK; ++k)
-            umma_fp8<2>(tmem_base + as * kBN, adesc0 + soff + 2u * k, bdesc0 + soff + 2u * k, idesc, k > 0);
-          umma_commit<2>(empty_bar(stage));
-          umma_commit<2>(acc_full_bar(as));
-          if (++stage == T::kStages) {
-            stage = 0;
-            parity ^= 1u;
+            for (int h = 0; h < T::kParts; ++h) {
+              if (h == 0) {
+                bool acc_ok, full_ok;
+                mbar_try_wait_both(acc_empty_bar(as), acc_parity, full_bar(stage), parity, acc_ok, full_ok);
+                if (!acc_ok) mbar_wait_inline(acc_empty_bar(as), acc_parity, ctl, kCodeMmaAcc);
+                if (!full_ok) mbar_wait_inline(full_bar(stage), parity, ctl, kCodeMmaFull);
+              } else {
+                mbar_wait_inline(acc_empty_bar(as), acc_parity, ctl, kCodeMmaAcc);
+              }
+              tcgen05_fence_after();
+              if (elect_one()) {
+#pragma unroll
+                for (int k = 0; k < kBlock / kSliceK; ++k)
+                  umma_fp8<2>(tmem_base + as * T::kAccCols, adesc0 + soff + 2u * k,
+                              bdesc0 + soff + (h * 64 * kBlock >> 4) + 2u * k, idesc, k > 0);
+                umma_commit<2>(acc_full_bar(as));
+                if (h + 1 == T::kParts) umma_commit<2>(empty_bar(stage));
+              }
+              __syncwarp();
+              if (++as == T::kAcc) {
+                as = 0;
+                acc_parity ^= 1u;
+              }
+            }
+            if (++stage == T::kStages) {
+              stage = 0;
+              parity ^= 1u;
+            }
           }
-          if (++as == T::kAcc) {
-            as = 0;
-            acc_parity ^= 1u;
+        }
+      }
+    } else {
+      // ---------------------------------------------------------------- scales
+      // a's scale times b's for every row and both warpgroups' columns, kGroup blocks at a time:
+      // slot[block][warpgroup][row].  Read by the read-back warps themselves, their latency showed up
+      // in every second block.
+      const int r = threadIdx.x - 64;
+      uint32_t slot = 0, wait_parity = 1;
+      for (int t = pair; t < p.num_tiles; t += num_pairs) {
+        int tm, tn;
+        tile_at(t, tm, tn);
+        const int row0 = tm * 2 * kTileRows + static_cast<int>(cta_rank) * kTileRows + r;
+        const float* sa0 = p.a.p + min(row0, p.m - 1) * p.a.row;
+        const float* sa1 = p.a.p + min(row0 + 64, p.m - 1) * p.a.row;
+        const float* sb0 = p.b.p + (min(tn * kBN, p.n - 1) / kBlock) * p.b.row;
+        const float* sb1 = p.b.p + (min(tn * kBN + T::kCols, p.n - 1) / kBlock) * p.b.row;
+        for (int kb0 = 0; kb0 < p.k_blocks; kb0 += T::kGroup) {
+          float a0[T::kGroup], a1[T::kGroup], b0[T::kGroup], b1[T::kGroup];
+#pragma unroll
+          for (int i = 0; i < T::kGroup; ++i) {
+            const int kb = min(kb0 + i, p.k_blocks - 1);
+            a0[i] = __ldg(sa0 + kb * p.a.blk);
+            a1[i] = __ldg(sa1 + kb * p.a.blk);
+            b0[i] = __ldg(sb0 + kb * p.b.blk);
+            b1[i] = __ldg(sb1 + kb * p.b.blk);
+          }
+          mbar_wait_inline(scale_empty_bar(slot), wait_parity, ctl, kCodeProducer);
+          float* dst = scales + slot * T::kSlotFloats + r;
+#pragma unroll
+          for (int i = 0; i < T::kGroup; ++i) {
+            dst[(2 * i) * kTileRows] = a0[i] * b0[i];
+            dst[(2 * i) * kTileRows + 64] = a1[i] * b0[i];
+            dst[(2 * i + 1) * kTileRows] = a0[i] * b1[i];
+            dst[(2 * i + 1) * kTileRows + 64] = a1[i] * b1[i];
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(scale_full_bar(slot));
+          if (++slot == T::kSlots) {
+            slot = 0;
+            wait_parity ^= 1u;
           }
         }
       }
     }
     __syncwarp();
   } else {
-    regs_inc<224>();
+    regs_inc<232>();
     // ---------------------------------------------------------------- read-back
     const int quarter = warp & 3;
     const int wg = (warp >> 2) - 1;
     const uint32_t acc_empty_leader = mapa_shared(acc_empty_bar(0), 0);
-    const uint32_t lane_addr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + wg * T::kCols;
+    const uint32_t lane_addr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + wg * 64;
     const uint32_t buf = store_base + (warp - 4) * T::kStoreBytes;
-    uint32_t as = 0, acc_parity = 0;
+    const float* my_scale = scales + wg * kTileRows + quarter * 32 + lane;
+    uint32_t as = 0, acc_parity = 0, slot = 0, slot_parity = 0;
     for (int t = pair; t < p.num_tiles; t += num_pairs) {
-      int tm, tn;
-      tile_at(t, tm, tn);
-      const int row0 = tm * 2 * kTileRows + static_cast<int>(cta_rank) * kTileRows + quarter * 32;
-      const int col0 = tn * kBN + wg * T::kCols;
-      const float* sa = p.a.p + min(row0 + lane, p.m - 1) * p.a.row;
-      const float* sb = p.b.p + (min(col0, p.n - 1) / kBlock) * p.b.row;
       uint64_t acc[T::kCols / 2];
 #pragma unroll
       for (int j = 0; j < T::kCols / 2; ++j) acc[j] = 0;
-      // the scales of four blocks are fetched while the four before them are used
-      constexpr int kAhead = 4;
-      float na[kAhead], nb[kAhead];
+      // A stage's 64 columns come in two loads of 32.  Each load is issued before the one in front of
+      // it is used, across the stages of a tile, since the wait is for all loads in flight.
+      uint32_t v[2][32];
+      mbar_wait_inline(acc_full_bar(as), acc_parity, ctl, kCodeEpilogue);
+      tcgen05_fence_after();
+      tmem_ld_32x32(lane_addr + as * T::kAccCols, v[0]);
+      for (int kb0 = 0; kb0 < p.k_blocks; kb0 += T::kGroup) {
+        mbar_wait_inline(scale_full_bar(slot), slot_parity, ctl, kCodeEpilogue);
+        float sc[T::kGroup];
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i) {
-        const int kb = min(i, p.k_blocks - 1);
-        na[i] = __ldg(sa + kb * p.a.blk);
-        nb[i] = __ldg(sb + kb * p.b.blk);
-      }
-      for (int kb0 = 0; kb0 < p.k_blocks; kb0 += kAhead) {
-        float sc[kAhead];
-#pragma unroll
-        for (int i = 0; i < kAhead; ++i) sc[i] = na[i] * nb[i];
-#pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
-          const int kb = min(kb0 + kAhead + i, p.k_blocks - 1);
-          na[i] = __ldg(sa + kb * p.a.blk);
-          nb[i] = __ldg(sb + kb * p.b.blk);
+        for (int i = 0; i < T::kGroup; ++i) sc[i] = my_scale[slot * T::kSlotFloats + 2 * i * kTileRows];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(scale_empty_bar(slot));
+        if (++slot == T::kSlots) {
+          slot = 0;
+          slot_parity ^= 1u;
         }
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
+        for (int i = 0; i < T::kGroup; ++i) {
           if (kb0 + i < p.k_blocks) {
-            mbar_wait_inline(acc_full_bar(as), acc_parity, ctl, kCodeEpilogue);
-            tcgen05_fence_after();
             const uint64_t s2 = pack_f32x2(__float_as_uint(sc[i]), __float_as_uint(sc[i]));
-            constexpr int kChunks = T::kCols / 16;
-            uint32_t v[2][16];
-            tmem_ld_32x16(lane_addr + as * kBN, v[0]);
 #pragma unroll
-            for (int c = 0; c < kChunks; ++c) {
-              tmem_ld_wait(v[c & 1]);
-              if (c + 1 < kChunks) tmem_ld_32x16(lane_addr + as * kBN + (c + 1) * 16, v[(c + 1) & 1]);
-              if (c + 1 == kChunks) {       // everything is in registers: the stage is free
-                tcgen05_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive_cluster_relaxed(acc_empty_leader + 8u * as);
+            for (int h = 0; h < T::kParts; ++h) {
+              tmem_ld_wait(v[0]);
+              tmem_ld_32x32(lane_addr + as * T::kAccCols + 32, v[1]);
+#pragma unroll
+              for (int j = 0; j < 16; ++j)
+                acc[h * 32 + j] = fma_f32x2(pack_f32x2(v[0][2 * j], v[0][2 * j + 1]), s2, acc[h * 32 + j]);
+              tmem_ld_wait(v[1]);
+              tcgen05_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive_cluster_relaxed(acc_empty_leader + 8u * as);
+              if (++as == T::kAcc) {
+                as = 0;
+                acc_parity ^= 1u;
+              }
+              if (h + 1 < T::kParts || kb0 + i + 1 < p.k_blocks) {
+                mbar_wait_inline(acc_full_bar(as), acc_parity, ctl, kCodeEpilogue);
+                tcgen05_fence_after();
+                tmem_ld_32x32(lane_addr + as * T::kAccCols, v[0]);
               }
 #pragma unroll
-              for (int j = 0; j < 8; ++j)
-                acc[c * 8 + j] = fma_f32x2(pack_f32x2(v[c & 1][2 * j], v[c & 1][2 * j + 1]), s2, acc[c * 8 + j]);
-            }
-            if (++as == T::kAcc) {
-              as = 0;
-              acc_parity ^= 1u;
+              for (int j = 0; j < 16; ++j)
+                acc[h * 32 + 16 + j] = fma_f32x2(pack_f32x2(v[1][2 * j], v[1][2 * j + 1]), s2, acc[h * 32 + 16 + j]);
             }
           }
         }
       }
       // bf16, 64 columns at a time through this warp's staging buffer
+      int tm, tn;
+      tile_at(t, tm, tn);
+      const int row0 = tm * 2 * kTileRows + static_cast<int>(cta_rank) * kTileRows + quarter * 32;
+      const int col0 = tn * kBN + wg * T::kCols;
 #pragma unroll
       for (int h = 0; h < T::kCols / 64; ++h) {
         if (lane == 0) bulk_wait_group_read<0>();
@@ -357,7 +441,8 @@ k_gemm_fp8_few(const __grid_constant__ CUtensorMap tma_w, const __grid_constant_
   const uint32_t misc = bar_base + 8u * (2 * T::kStages + 2 * T::kAcc);
   volatile uint32_t* misc_gen = reinterpret_cast<volatile uint32_t*>(smem_raw + (misc - raw));
 
-  const int warp = threadIdx.x >> 5;
+  // warp-uniform by construction, so that the single-thread roles keep their state in uniform registers
+  const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
   const int lane = threadIdx.x & 31;
   const int rank = p.split > 1 ? static_cast<int>(cluster_ctarank()) : 0;
   const int tile = blockIdx.x / p.split;
@@ -390,51 +475,51 @@ k_gemm_fp8_few(const __grid_constant__ CUtensorMap tma_w, const __grid_constant_
   tcgen05_fence_before();
   __syncthreads();
   tcgen05_fence_after();
-  const uint32_t tmem_base = misc_gen[0];
+  const uint32_t tmem_base = __shfl_sync(0xffffffffu, misc_gen[0], 0);
 
   if (warp == 0) {
-    if (lane == 0) {
-      uint32_t stage = 0, wait_parity = 1;
-      for (int kb = kb0; kb < kb1; ++kb) {
-        mbar_wait_inline(empty_bar(stage), wait_parity, ctl, kCodeProducer);
+    uint32_t stage = 0, wait_parity = 1;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      mbar_wait_inline(empty_bar(stage), wait_parity, ctl, kCodeProducer);
+      if (elect_one()) {
         mbar_arrive_expect_tx(full_bar(stage), T::kStageBytes);
         const uint32_t sw = base + stage * T::kStageBytes;
         tma_load_2d(sw, &tma_w, full_bar(stage), kb * kBlock, n0);
         tma_load_2d(sw + kOperandBytes, &tma_x, full_bar(stage), kb * kBlock, m0);
-        if (++stage == T::kStages) {
-          stage = 0;
-          wait_parity ^= 1u;
-        }
+      }
+      __syncwarp();
+      if (++stage == T::kStages) {
+        stage = 0;
+        wait_parity ^= 1u;
       }
     }
-    __syncwarp();
   } else if (warp == 1) {
-    if (lane == 0) {
-      constexpr uint32_t idesc = make_idesc_e4m3(kTileRows, kBT);
-      const uint64_t wdesc0 = make_kmajor_sw128_desc(base);
-      const uint64_t xdesc0 = make_kmajor_sw128_desc(base + kOperandBytes);
-      uint32_t stage = 0, parity = 0, as = 0, acc_parity = 1;
-      for (int kb = kb0; kb < kb1; ++kb) {
-        mbar_wait_inline(acc_empty_bar(as), acc_parity, ctl, kCodeMmaAcc);
-        mbar_wait_inline(full_bar(stage), parity, ctl, kCodeMmaFull);
-        tcgen05_fence_after();
-        const uint64_t soff = static_cast<uint64_t>(stage * (T::kStageBytes >> 4));
+    constexpr uint32_t idesc = make_idesc_e4m3(kTileRows, kBT);
+    const uint64_t wdesc0 = make_kmajor_sw128_desc(base);
+    const uint64_t xdesc0 = make_kmajor_sw128_desc(base + kOperandBytes);
+    uint32_t stage = 0, parity = 0, as = 0, acc_parity = 1;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      mbar_wait_inline(acc_empty_bar(as), acc_parity, ctl, kCodeMmaAcc);
+      mbar_wait_inline(full_bar(stage), parity, ctl, kCodeMmaFull);
+      tcgen05_fence_after();
+      const uint64_t soff = static_cast<uint64_t>(stage * (T::kStageBytes >> 4));
+      if (elect_one()) {
 #pragma unroll
         for (int k = 0; k < kBlock / kSliceK; ++k)
           umma_fp8<1>(tmem_base + as * kBT, wdesc0 + soff + 2u * k, xdesc0 + soff + 2u * k, idesc, k > 0);
-        umma_commit<1>(empty_bar(stage));
         umma_commit<1>(acc_full_bar(as));
-        if (++stage == T::kStages) {
-          stage = 0;
-          parity ^= 1u;
-        }
-        if (++as == T::kAcc) {
-          as = 0;
-          acc_parity ^= 1u;
-        }
+        umma_commit<1>(empty_bar(stage));
+      }
+      __syncwarp();
+      if (++stage == T::kStages) {
+        stage = 0;
+        parity ^= 1u;
+      }
+      if (++as == T::kAcc) {
+        as = 0;
+        acc_parity ^= 1u;
       }
     }
-    __syncwarp();
   } else {
     // ---------------------------------------------------------------- read-back
     const int quarter = warp & 3;

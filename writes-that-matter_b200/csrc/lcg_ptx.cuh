@@ -97,6 +97,25 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
   return ok != 0;
 }
 
+// Two waits tried together: one round trip when both have been met.
+__device__ __forceinline__ void mbar_try_wait_both(uint32_t bar0, uint32_t parity0, uint32_t bar1, uint32_t parity1,
+                                                   bool& ok0, bool& ok1) {
+  uint32_t a, b;
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p, q;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%2], %3;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 q, [%4], %5;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "selp.u32 %1, 1, 0, q;\n\t"
+      "}\n"
+      : "=r"(a), "=r"(b)
+      : "r"(bar0), "r"(parity0), "r"(bar1), "r"(parity1)
+      : "memory");
+  ok0 = a != 0;
+  ok1 = b != 0;
+}
+
 // Per-CTA control block for bounded waits.  `abort_flag` lives in shared
 // memory; once any wait of the CTA has run out it is set and every later wait
 // returns at once, so the kernel's control flow (loop trip counts, named
@@ -135,11 +154,14 @@ __device__ __forceinline__ void mbar_wait(uint32_t bar, uint32_t parity, const W
 // The same without a call: for warps whose registers are full of accumulators, which a call's
 // register convention would move about.
 __device__ __forceinline__ void mbar_wait_inline(uint32_t bar, uint32_t parity, const WaitCtl& ctl, int code) {
-  if (mbar_try_wait(bar, parity)) return;
-  const uint64_t t0 = globaltimer_ns();
-  while (!mbar_try_wait(bar, parity)) {
+  uint64_t t0 = 0;
+  // the timer is read once in 64 tries: reading it takes longer than most waits
+  for (uint32_t tries = 1; !mbar_try_wait(bar, parity); ++tries) {
+    if ((tries & 63u) != 0) continue;
     if (*ctl.abort_flag) return;
-    if (globaltimer_ns() - t0 > ctl.limit_ns) {
+    const uint64_t now = globaltimer_ns();
+    if (t0 == 0) t0 = now;
+    if (now - t0 > ctl.limit_ns) {
       *ctl.abort_flag = 1u;
       if (ctl.status != nullptr) atomicCAS(ctl.status, 0, code);
       return;
@@ -398,6 +420,17 @@ __device__ __forceinline__ void tmem_ld_32x32(uint32_t taddr, uint32_t (&r)[32])
       : "memory");
 }
 
+// Wait for the loads in flight, naming the registers of one of them: what uses them stays behind it.
+__device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                 "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+                 "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+               :
+               : "memory");
+}
+
 // The same, 16 columns.
 __device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
@@ -410,7 +443,6 @@ __device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, uint32_t (&r)[16])
       : "memory");
 }
 
-// Wait for the loads in flight, naming the registers of one of them: what uses them stays behind it.
 __device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[16]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;"
                : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
