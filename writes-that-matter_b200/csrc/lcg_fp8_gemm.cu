@@ -52,20 +52,11 @@ __device__ __forceinline__ void regs_dec() {
 constexpr int kCodeProducer = 101, kCodeMmaAcc = 102, kCodeMmaFull = 103, kCodeEpilogue = 104;
 
 // ================================================================ many rows
-// A pair multiplies 256 rows of a by kBN rows of b, 128 columns of the accumulator at a time: TMEM
-// holds four stages of 128 columns, so that a block's sums stay there while they are read back and
-// the next ones are being formed.  (Two stages of 256 columns would take half as many instructions, but
-// a stage is then handed back so late that the tensor cores wait for it.)
-//
 // 12 warps: 0 TMA producer, 1 MMA issuer, 2 and 3 scales, 4-7 and 8-11 read-back: every warp one
-// TMEM lane quarter, each warpgroup half of a stage's columns.  Columns [0, 64) of stage h of a
-// tile come from rows 64 h .. of the b tile in CTA 0 and columns [64, 128) from CTA 1's, so
-// warpgroup w owns columns [w * kBN / 2, (w + 1) * kBN / 2) of the tile.
+// TMEM lane quarter, each warpgroup half of the columns.
 template <int kBN>
 struct Many {
-  static constexpr int kAccCols = 128;
-  static constexpr int kAcc = 512 / kAccCols;               // TMEM stages
-  static constexpr int kParts = kBN / kAccCols;             // stages a K block fills
+  static constexpr int kAcc = 512 / kBN;                    // TMEM stages
   static constexpr int kBRows = kBN / 2;                    // rows of b each CTA of the pair loads
   static constexpr int kStageBytes = kOperandBytes + kBRows * kBlock;
   static constexpr int kStages = kBN == 256 ? 5 : 7;
@@ -191,37 +182,29 @@ k_gemm_fp8(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CU
       // uniform registers.  With one lane in the loop every instruction first moved its operands
       // there, 75 cycles for each MMA, more than the MMA takes.
       if (leader) {
-        constexpr uint32_t idesc = make_idesc_e4m3(2 * kTileRows, T::kAccCols);
+        constexpr uint32_t idesc = make_idesc_e4m3(2 * kTileRows, kBN);
         const uint64_t adesc0 = make_kmajor_sw128_desc(base);
         const uint64_t bdesc0 = make_kmajor_sw128_desc(base + kOperandBytes);
         uint32_t stage = 0, parity = 0, as = 0, acc_parity = 1;
         for (int t = pair; t < p.num_tiles; t += num_pairs) {
           for (int kb = 0; kb < p.k_blocks; ++kb) {
             const uint64_t soff = static_cast<uint64_t>(stage * (T::kStageBytes >> 4));
+            bool acc_ok, full_ok;
+            mbar_try_wait_both(acc_empty_bar(as), acc_parity, full_bar(stage), parity, acc_ok, full_ok);
+            if (!acc_ok) mbar_wait_inline(acc_empty_bar(as), acc_parity, ctl, kCodeMmaAcc);
+            if (!full_ok) mbar_wait_inline(full_bar(stage), parity, ctl, kCodeMmaFull);
+            tcgen05_fence_after();
+            if (elect_one()) {
 #pragma unroll
-            for (int h = 0; h < T::kParts; ++h) {
-              if (h == 0) {
-                bool acc_ok, full_ok;
-                mbar_try_wait_both(acc_empty_bar(as), acc_parity, full_bar(stage), parity, acc_ok, full_ok);
-                if (!acc_ok) mbar_wait_inline(acc_empty_bar(as), acc_parity, ctl, kCodeMmaAcc);
-                if (!full_ok) mbar_wait_inline(full_bar(stage), parity, ctl, kCodeMmaFull);
-              } else {
-                mbar_wait_inline(acc_empty_bar(as), acc_parity, ctl, kCodeMmaAcc);
-              }
-              tcgen05_fence_after();
-              if (elect_one()) {
-#pragma unroll
-                for (int k = 0; k < kBlock / kSliceK; ++k)
-                  umma_fp8<2>(tmem_base + as * T::kAccCols, adesc0 + soff + 2u * k,
-                              bdesc0 + soff + (h * 64 * kBlock >> 4) + 2u * k, idesc, k > 0);
-                umma_commit<2>(acc_full_bar(as));
-                if (h + 1 == T::kParts) umma_commit<2>(empty_bar(stage));
-              }
-              __syncwarp();
-              if (++as == T::kAcc) {
-                as = 0;
-                acc_parity ^= 1u;
-              }
+              for (int k = 0; k < kBlock / kSliceK; ++k)
+                umma_fp8<2>(tmem_base + as * kBN, adesc0 + soff + 2u * k, bdesc0 + soff + 2u * k, idesc, k > 0);
+              umma_commit<2>(acc_full_bar(as));
+              umma_commit<2>(empty_bar(stage));
+            }
+            __syncwarp();
+            if (++as == T::kAcc) {
+              as = 0;
+              acc_parity ^= 1u;
             }
             if (++stage == T::kStages) {
               stage = 0;
@@ -280,7 +263,7 @@ k_gemm_fp8(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CU
     const int quarter = warp & 3;
     const int wg = (warp >> 2) - 1;
     const uint32_t acc_empty_leader = mapa_shared(acc_empty_bar(0), 0);
-    const uint32_t lane_addr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + wg * 64;
+    const uint32_t lane_addr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + wg * T::kCols;
     const uint32_t buf = store_base + (warp - 4) * T::kStoreBytes;
     const float* my_scale = scales + wg * kTileRows + quarter * 32 + lane;
     uint32_t as = 0, acc_parity = 0, slot = 0, slot_parity = 0;
@@ -288,12 +271,13 @@ k_gemm_fp8(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CU
       uint64_t acc[T::kCols / 2];
 #pragma unroll
       for (int j = 0; j < T::kCols / 2; ++j) acc[j] = 0;
-      // A stage's 64 columns come in two loads of 32.  Each load is issued before the one in front of
-      // it is used, across the stages of a tile, since the wait is for all loads in flight.
+      // Loads of 32 columns.  Each is issued before the one in front of it is used, across the stages
+      // of a tile too: the wait is for all of a warp's loads, so there is one in flight.
+      constexpr int kChunks = T::kCols / 32;
       uint32_t v[2][32];
       mbar_wait_inline(acc_full_bar(as), acc_parity, ctl, kCodeEpilogue);
       tcgen05_fence_after();
-      tmem_ld_32x32(lane_addr + as * T::kAccCols, v[0]);
+      tmem_ld_32x32(lane_addr + as * kBN, v[0]);
       for (int kb0 = 0; kb0 < p.k_blocks; kb0 += T::kGroup) {
         mbar_wait_inline(scale_full_bar(slot), slot_parity, ctl, kCodeEpilogue);
         float sc[T::kGroup];
@@ -310,28 +294,27 @@ k_gemm_fp8(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CU
           if (kb0 + i < p.k_blocks) {
             const uint64_t s2 = pack_f32x2(__float_as_uint(sc[i]), __float_as_uint(sc[i]));
 #pragma unroll
-            for (int h = 0; h < T::kParts; ++h) {
-              tmem_ld_wait(v[0]);
-              tmem_ld_32x32(lane_addr + as * T::kAccCols + 32, v[1]);
+            for (int c = 0; c < kChunks; ++c) {
+              tmem_ld_wait(v[c & 1]);
+              if (c + 1 < kChunks) {
+                tmem_ld_32x32(lane_addr + as * kBN + (c + 1) * 32, v[(c + 1) & 1]);
+              } else {          // everything is in registers: the stage goes back, the next one begins
+                tcgen05_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster_relaxed(acc_empty_leader + 8u * as);
+                if (++as == T::kAcc) {
+                  as = 0;
+                  acc_parity ^= 1u;
+                }
+                if (kb0 + i + 1 < p.k_blocks) {
+                  mbar_wait_inline(acc_full_bar(as), acc_parity, ctl, kCodeEpilogue);
+                  tcgen05_fence_after();
+                  tmem_ld_32x32(lane_addr + as * kBN, v[0]);
+                }
+              }
 #pragma unroll
               for (int j = 0; j < 16; ++j)
-                acc[h * 32 + j] = fma_f32x2(pack_f32x2(v[0][2 * j], v[0][2 * j + 1]), s2, acc[h * 32 + j]);
-              tmem_ld_wait(v[1]);
-              tcgen05_fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive_cluster_relaxed(acc_empty_leader + 8u * as);
-              if (++as == T::kAcc) {
-                as = 0;
-                acc_parity ^= 1u;
-              }
-              if (h + 1 < T::kParts || kb0 + i + 1 < p.k_blocks) {
-                mbar_wait_inline(acc_full_bar(as), acc_parity, ctl, kCodeEpilogue);
-                tcgen05_fence_after();
-                tmem_ld_32x32(lane_addr + as * T::kAccCols, v[0]);
-              }
-#pragma unroll
-              for (int j = 0; j < 16; ++j)
-                acc[h * 32 + 16 + j] = fma_f32x2(pack_f32x2(v[1][2 * j], v[1][2 * j + 1]), s2, acc[h * 32 + 16 + j]);
+                acc[c * 16 + j] = fma_f32x2(pack_f32x2(v[c & 1][2 * j], v[c & 1][2 * j + 1]), s2, acc[c * 16 + j]);
             }
           }
         }
