@@ -383,7 +383,7 @@ int lcg_gemm_fp8(const void* a, int64_t lda, const float* a_scale, int64_t a_sca
                  int64_t M, int64_t N, int64_t K, int32_t* status, void* stream);
 
 /* ---- log probabilities ----------------------------------------------------
- * For each row of logits (M, V), leading dimension ld, of type bf16, fp16 or fp32:
+ * For each row of logits (M, V), V <= 2^20, leading dimension ld, of type bf16, fp16 or fp32:
  *   logprob = x[token] - ln(sum e^x)       entropy = -sum p ln p
  * and the `top` (0..32, at most V) largest values with their log probabilities, largest first,
  * equal values by rising id.  tokens: M ids of token_bytes (4 or 8) bytes each.  A masked value

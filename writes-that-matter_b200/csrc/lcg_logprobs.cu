@@ -1,105 +1,524 @@
-// Log probabilities of given tokens, the entropy of each row, and its most likely tokens.
+// Log probabilities of given tokens, the entropy of each row, and its most likely tokens, in one
+// pass over the logits.
 //
 // With m = max x, S = sum e^(x - m) and T = sum e^(x - m) (x - m) over a row (a masked value, -inf,
-// adds nothing to either):  log p(token) = (x[token] - m) - ln S,  H = ln S - T / S.
+// adds nothing to either):  log p(token) = (x[token] - m) - ln S,  H = ln S - T / S.  The pass keeps a
+// running m and rescales S and T when it grows.
+//
+// Alternatives.  A segment is what one warp reads in one load (32 vectors of 16 bytes).  The pass
+// leaves each segment's maximum in shared memory.  Of any partition into runs of consecutive ids, the
+// `top` best values (larger first, lower id first among equals) lie in the `top` best runs by the
+// same order of their maxima: a run outside has `top` runs before it, each with a value that comes
+// before all of its own.  So the `top` best segments are read again, of those the `top` best vectors are
+// kept, and of their at most 256 values each is ranked by counting.  The cost does not depend on the
+// values: no order of the row and no number of ties makes it longer.
+//
+// Bound by HBM for many rows (2 or 4 bytes a value; the exponential unit is at 3/4 of its rate on bf16), by the
+// latency of the selection for one row.  A row is one CTA's, or a cluster's of up to eight when there
+// are too few rows to fill the GPU; the CTAs' parts are joined through distributed shared memory in
+// rank order, so the result does not depend on timing.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <math_constants.h>
 
 #include "lcg_common.h"
+#include "lcg_ptx.cuh"
 
 namespace lcg {
 namespace {
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 256;
+constexpr int kWarps = kThreads / 32;
 constexpr int kMaxTop = 32;
+constexpr int kMaxCluster = 8;
+constexpr int64_t kMaxColumns = 1 << 20;     // a row's segment maxima then take at most 32 KiB
+constexpr int kUnroll = 4;                   // 16-byte loads of a thread in flight
 
+// -------------------------------------------------------------------- values
+template <typename T>
+struct Vec;
+template <>
+struct Vec<float> {
+  static constexpr int kN = 4;
+  __device__ static void unpack(const uint4& q, float (&f)[4]) {
+    f[0] = __uint_as_float(q.x), f[1] = __uint_as_float(q.y), f[2] = __uint_as_float(q.z), f[3] = __uint_as_float(q.w);
+  }
+  __device__ static float max(const uint4& q) {
+    return fmaxf(fmaxf(__uint_as_float(q.x), __uint_as_float(q.y)), fmaxf(__uint_as_float(q.z), __uint_as_float(q.w)));
+  }
+};
+template <>
+struct Vec<__nv_bfloat16> {
+  static constexpr int kN = 8;
+  __device__ static void unpack(const uint4& q, float (&f)[8]) {
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      f[2 * t] = __uint_as_float(w[t] << 16);
+      f[2 * t + 1] = __uint_as_float(w[t] & 0xffff0000u);
+    }
+  }
+  __device__ static float max(const uint4& q) {
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&q);
+    const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+    return fmaxf(__low2float(m), __high2float(m));
+  }
+};
+template <>
+struct Vec<__half> {
+  static constexpr int kN = 8;
+  __device__ static void unpack(const uint4& q, float (&f)[8]) {
+    const __half2* h = reinterpret_cast<const __half2*>(&q);
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const float2 v = __half22float2(h[t]);
+      f[2 * t] = v.x;
+      f[2 * t + 1] = v.y;
+    }
+  }
+  __device__ static float max(const uint4& q) {
+    const __half2* h = reinterpret_cast<const __half2*>(&q);
+    const __half2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+    return fmaxf(__low2float(m), __high2float(m));
+  }
+};
 __device__ __forceinline__ float to_float(float v) { return v; }
 __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
 __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T>
+__device__ __forceinline__ uint32_t minus_inf_bits();
+template <>
+__device__ __forceinline__ uint32_t minus_inf_bits<float>() { return 0xff800000u; }
+template <>
+__device__ __forceinline__ uint32_t minus_inf_bits<__half>() { return 0xfc00u; }
+template <>
+__device__ __forceinline__ uint32_t minus_inf_bits<__nv_bfloat16>() { return 0xff80u; }
 
-// Order of the alternatives: larger value first, lower id first among equals (0 and -0 alike); a
-// NaN counts as -inf there (a row that holds one has no log probabilities at all).
+// Largest value of a warp, NaN left out.
+__device__ __forceinline__ float warp_max(float v) {
+  float r;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float ex2(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {     // a NaN stays one
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+  return pack_f32x2(__float_as_uint(lo), __float_as_uint(hi));
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// Order of the alternatives as whole numbers: larger is better, 0 and -0 alike, NaN with -inf; 0 is
+// no value's.
 __device__ __forceinline__ uint32_t order_key(float v) {
   v = v + 0.0f;
   if (v != v) v = -CUDART_INF_F;
   const uint32_t b = __float_as_uint(v);
   return (b & 0x80000000u) ? ~b : b | 0x80000000u;
 }
-__device__ __forceinline__ unsigned long long full_key(float v, uint32_t id) {
-  return (static_cast<unsigned long long>(order_key(v)) << 32) | (0xffffffffu - id);
+__device__ __forceinline__ float key_value(uint32_t key) {
+  return __uint_as_float((key & 0x80000000u) ? key & 0x7fffffffu : ~key);
 }
 
-__device__ float block_max(float v, float* s) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = s[0];
-  for (int w = 1; w < kThreads / 32; ++w) v = fmaxf(v, s[w]);
-  return v;
+// A running maximum with the sums that go with it; T in units of ln 2, as the exponentials are taken
+// to the base 2.
+struct Sums {
+  float m, s, t;
+};
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+// S and T of `a` seen from the maximum m >= a.m (the difference of two -inf is taken as 0).
+__device__ __forceinline__ void rescale(Sums& a, float m) {
+  const float d = a.m == m ? 0.f : (a.m - m) * kLog2e;
+  const float f = ex2(d);
+  a.t = a.s == 0.f ? 0.f : f == 0.f ? 0.f : f * fmaf(a.s, d, a.t);
+  a.s = a.s * f;
+  a.m = m;
 }
-__device__ float block_sum(float v, float* s) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = 0.f;
-  for (int w = 0; w < kThreads / 32; ++w) v += s[w];
-  return v;
+__device__ __forceinline__ Sums join(Sums a, Sums b) {
+  const float m = fmaxf(a.m, b.m);
+  rescale(a, m);
+  rescale(b, m);
+  return Sums{m, a.s + b.s, a.t + b.t};
 }
 
-// One CTA per row, one pass for the maximum, one for the sums, one for each alternative.
+// ---------------------------------------------------------------- one row
 template <typename T>
-__global__ void __launch_bounds__(kThreads)
-k_token_logprobs(const T* __restrict__ logits, int64_t V, int64_t ld, const void* __restrict__ tokens, int token_bytes,
-                 int top, float* __restrict__ logprob, float* __restrict__ entropy, float* __restrict__ top_logprobs,
-                 int64_t* __restrict__ top_ids) {
-  __shared__ float s_red[32];
-  __shared__ unsigned long long s_key[32];
-  const int64_t row = blockIdx.x;
-  const T* x = logits + row * ld;
-  float m = -CUDART_INF_F;
-  for (int64_t i = threadIdx.x; i < V; i += kThreads) m = fmaxf(m, to_float(x[i]));
-  m = block_max(m, s_red);
-  float S = 0.f, Tm = 0.f;
-  for (int64_t i = threadIdx.x; i < V; i += kThreads) {
-    const float v = to_float(x[i]);
-    const float y = v - m;          // NaN where the row is all -inf, or holds +inf or NaN
-    const float e = expf(y);
-    S += e;
-    if (v != -CUDART_INF_F && e != 0.f) Tm = fmaf(e, y, Tm);
+struct Row {
+  static constexpr int kN = Vec<T>::kN;
+  const T* x;          // the row
+  const uint4* grid;   // the 16-byte grid that covers it
+  int head;            // values of the first vector in front of the row
+  int V;
+  int full0, full1;    // vectors [full0, full1) lie inside the row
+  __device__ Row(const T* row, int v) : x(row), V(v) {
+    const uintptr_t p = reinterpret_cast<uintptr_t>(row);
+    head = static_cast<int>((p & 15u) / sizeof(T));
+    grid = reinterpret_cast<const uint4*>(p & ~uintptr_t(15));
+    full0 = head > 0 ? 1 : 0;
+    full1 = (V + head) / kN;
   }
-  S = block_sum(S, s_red);
-  Tm = block_sum(Tm, s_red);
-  const float lse = logf(S);
-  if (threadIdx.x == 0) {
-    const int64_t t = token_bytes == 8 ? static_cast<const int64_t*>(tokens)[row] : static_cast<const int32_t*>(tokens)[row];
-    logprob[row] = t >= 0 && t < V ? (to_float(x[t]) - m) - lse : __int_as_float(0x7fc00000);
-    entropy[row] = lse - Tm / S;
-  }
-  unsigned long long last = ~0ull;
-  for (int k = 0; k < top; ++k) {
-    unsigned long long best = 0;
-    for (int64_t i = threadIdx.x; i < V; i += kThreads) {
-      const unsigned long long key = full_key(to_float(x[i]), static_cast<uint32_t>(i));
-      if (key < last && key > best) best = key;
-    }
+  __device__ int vectors() const { return (V + head + kN - 1) / kN; }
+  // Vector i with -inf outside the row; only what lies inside is read.
+  __device__ uint4 load(int i) const {
+    if (i >= full0 && i < full1) return __ldg(grid + i);
+    constexpr int kPerWord = 4 / static_cast<int>(sizeof(T));
+    uint32_t w[4];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) s_key[threadIdx.x >> 5] = best;
-    __syncthreads();
-    for (int w = 0; w < kThreads / 32; ++w) best = max(best, s_key[w]);
-    last = best;
-    if (threadIdx.x == 0) {
-      const uint32_t id = 0xffffffffu - static_cast<uint32_t>(best);
-      top_ids[row * top + k] = id;
-      top_logprobs[row * top + k] = (to_float(x[id]) - m) - lse;
+    for (int j = 0; j < 4; ++j) {
+      w[j] = 0;
+#pragma unroll
+      for (int e = 0; e < kPerWord; ++e) {
+        const int id = i * kN - head + j * kPerWord + e;
+        uint32_t bits = minus_inf_bits<T>();
+        if (id >= 0 && id < V) {
+          if constexpr (sizeof(T) == 4)
+            bits = reinterpret_cast<const uint32_t*>(x)[id];
+          else
+            bits = reinterpret_cast<const unsigned short*>(x)[id];
+        }
+        w[j] |= bits << (16 * e);
+      }
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+};
+
+// The k-th best of keys[0, n) (n >= k), and among values equal to it the ids below `limit` are in:
+// then exactly k of the keys satisfy chosen().  id_of gives the ids, which differ.  All threads call it.
+struct Cut {
+  uint32_t key, limit;
+  __device__ bool chosen(uint32_t k, uint32_t id) const { return k > key || (k == key && id < limit); }
+};
+template <typename IdOf>
+__device__ Cut find_cut(const uint32_t* keys, int n, int k, IdOf id_of) {
+  auto count = [&](auto pred) {
+    int c = 0;
+    for (int i0 = 0; i0 < n; i0 += kThreads) {
+      const int i = i0 + static_cast<int>(threadIdx.x);
+      c += __syncthreads_count(i < n && pred(keys[i < n ? i : 0], i));
+    }
+    return c;
+  };
+  Cut cut{0u, 0xffffffffu};
+  for (int b = 31; b >= 0; --b) {
+    const uint32_t cand = cut.key | (1u << b);
+    if (count([&](uint32_t key, int) { return key >= cand; }) >= k) cut.key = cand;
+  }
+  const int better = count([&](uint32_t key, int) { return key > cut.key; });
+  const int ties = count([&](uint32_t key, int) { return key == cut.key; });
+  if (better + ties > k) {        // the largest limit that lets no more than k in
+    uint32_t limit = 0;
+    for (int b = 30; b >= 0; --b) {
+      const uint32_t cand = limit | (1u << b);
+      const int in = count([&](uint32_t key, int i) { return key == cut.key && static_cast<uint32_t>(id_of(i)) < cand; });
+      if (better + in <= k) limit = cand;
+    }
+    cut.limit = limit;
+  }
+  return cut;
+}
+
+struct Entry {
+  uint32_t key, id;
+};
+__device__ __forceinline__ bool before(const Entry& a, const Entry& b) {
+  return a.key > b.key || (a.key == b.key && a.id < b.id);
+}
+
+struct Params {
+  const void* logits;
+  const void* tokens;
+  int64_t ld;
+  int32_t V, top, token_bytes, cluster;
+  float *logprob, *entropy, *top_logprobs;
+  int64_t* top_ids;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 5)
+k_token_logprobs(const __grid_constant__ Params p) {
+  constexpr int kN = Vec<T>::kN;
+  extern __shared__ uint32_t s_keys[];             // segment maxima, as keys
+  __shared__ Sums s_sums[kWarps];
+  __shared__ Sums s_part;                          // this CTA's sums, read by rank 0
+  __shared__ Entry s_best[kMaxTop];                // this CTA's best, in order; read by rank 0
+  __shared__ int s_nbest;
+  __shared__ uint32_t s_run[kMaxTop];              // chosen segments, then chosen vectors
+  __shared__ uint32_t s_vec_key[kMaxTop * 32];
+  __shared__ Entry s_cand[kMaxCluster * kMaxTop];
+  __shared__ int s_count;
+
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int rank = p.cluster > 1 ? static_cast<int>(cluster_ctarank()) : 0;
+  const int64_t row = blockIdx.x / p.cluster;
+  const Row<T> r(static_cast<const T*>(p.logits) + row * p.ld, p.V);
+  const int nvec = r.vectors();
+  const int nseg = (nvec + 31) / 32;
+  const int seg0 = static_cast<int>(static_cast<int64_t>(nseg) * rank / p.cluster);
+  const int seg1 = static_cast<int>(static_cast<int64_t>(nseg) * (rank + 1) / p.cluster);
+
+  // the token's value is fetched now and used at the end
+  float xt = CUDART_NAN_F;
+  if (rank == 0 && tid == 0) {
+    const int64_t t = p.token_bytes == 8 ? static_cast<const int64_t*>(p.tokens)[row]
+                                         : static_cast<int64_t>(static_cast<const int32_t*>(p.tokens)[row]);
+    if (t >= 0 && t < p.V) xt = to_float(r.x[t]);
+  }
+
+  // ------------------------------------------------------------------ the pass
+  // m is the warp's: equal in its lanes.  S and T are each lane's own, two of each.
+  float m = -CUDART_INF_F;
+  uint64_t s2 = 0, t2 = 0;
+  const uint64_t scale2 = pair(kLog2e, kLog2e);
+  auto take = [&](const uint4 (&q)[kUnroll], int seg, int count) {
+    float mx[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) mx[u] = u < count ? warp_max(Vec<T>::max(q[u])) : -CUDART_INF_F;
+    if (p.top > 0 && lane == 0) {
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u)
+        if (u < count) s_keys[seg + u * kWarps - seg0] = order_key(mx[u]);
+    }
+    float grown = m;
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) grown = fmaxf(grown, mx[u]);
+    if (grown > m) {
+      float slo, shi, tlo, thi;
+      unpack_f32x2(s2, slo, shi);
+      unpack_f32x2(t2, tlo, thi);
+      Sums lo{m, slo, tlo}, hi{m, shi, thi};
+      rescale(lo, grown);
+      rescale(hi, grown);
+      s2 = pair(lo.s, hi.s);
+      t2 = pair(lo.t, hi.t);
+      m = grown;
+    }
+    const float minus_m = m == -CUDART_INF_F ? 0.f : -m;
+    const uint64_t shift2 = pair(minus_m, minus_m);
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      if (u < count) {
+        float f[kN];
+        Vec<T>::unpack(q[u], f);
+#pragma unroll
+        for (int e = 0; e < kN; e += 2) {
+          float lo, hi;
+          unpack_f32x2(mul2(add2(pair(f[e], f[e + 1]), shift2), scale2), lo, hi);
+          // a masked value's difference is -inf, which must not meet the 0 of its exponential
+          lo = max_nan(lo, -200.f);
+          hi = max_nan(hi, -200.f);
+          const uint64_t e2 = pair(ex2(lo), ex2(hi));
+          s2 = add2(s2, e2);
+          t2 = fma_f32x2(e2, pair(lo, hi), t2);
+        }
+      }
+    }
+  };
+  {
+    const int inner0 = (r.full0 + 31) / 32, inner1 = r.full1 / 32;    // segments that lie inside the row
+    int seg = seg0 + warp;
+    for (; seg + (kUnroll - 1) * kWarps < seg1; seg += kUnroll * kWarps) {
+      uint4 q[kUnroll];
+      if (seg >= inner0 && seg + (kUnroll - 1) * kWarps < inner1) {
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) q[u] = __ldg(r.grid + (seg + u * kWarps) * 32 + lane);
+      } else {
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) q[u] = r.load((seg + u * kWarps) * 32 + lane);
+      }
+      take(q, seg, kUnroll);
+    }
+    if (seg < seg1) {
+      uint4 q[kUnroll];
+      const int count = (seg1 - seg + kWarps - 1) / kWarps;
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u)
+        if (u < count) q[u] = r.load((seg + u * kWarps) * 32 + lane);
+      take(q, seg, count);
     }
   }
+  // Lanes, warps, CTAs: always in the same order.
+  {
+    float slo, shi, tlo, thi;
+    unpack_f32x2(s2, slo, shi);
+    unpack_f32x2(t2, tlo, thi);
+    float s = slo + shi, t = tlo + thi;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      s += __shfl_xor_sync(0xffffffffu, s, o);
+      t += __shfl_xor_sync(0xffffffffu, t, o);
+    }
+    if (lane == 0) s_sums[warp] = Sums{m, s, t};
+  }
+  if (tid == 0) {
+    s_count = 0;
+    s_nbest = 0;
+  }
+  __syncthreads();
+  if (tid == 0) {
+    Sums a = s_sums[0];
+    for (int w = 1; w < kWarps; ++w) a = join(a, s_sums[w]);
+    s_part = a;
+  }
+
+  // -------------------------------------------------------------- alternatives
+  const int first = max(0, seg0 * 32 * kN - r.head);
+  const int last = min(r.V, seg1 * 32 * kN - r.head);
+  const int want = min(p.top, last - first);        // of this CTA's part of the row
+  if (want > 0) {
+    const int n = seg1 - seg0;
+    const int runs = min(want, n);
+    const Cut seg_cut = find_cut(s_keys, n, runs, [&](int i) { return i; });
+    for (int i = tid; i < n; i += kThreads)
+      if (seg_cut.chosen(s_keys[i], i)) s_run[atomicAdd(&s_count, 1)] = seg0 + i;
+    __syncthreads();
+    // every vector of the chosen segments: its best value, 0 where it holds none of the row
+    const int nv = runs * 32;
+    for (int i = tid; i < nv; i += kThreads) {
+      const int v = static_cast<int>(s_run[i >> 5]) * 32 + (i & 31);
+      uint32_t key = 0;
+      if (v < nvec) {
+        float f[kN];
+        Vec<T>::unpack(r.load(v), f);
+#pragma unroll
+        for (int e = 0; e < kN; ++e) {
+          const int id = v * kN - r.head + e;
+          if (id >= 0 && id < r.V) key = max(key, order_key(f[e]));
+        }
+      }
+      s_vec_key[i] = key;
+    }
+    if (tid == 0) s_count = 0;
+    __syncthreads();
+    const int vecs = min(want, nv);
+    auto vec_id = [&](int i) { return static_cast<int>(s_run[i >> 5]) * 32 + (i & 31); };
+    const Cut vec_cut = find_cut(s_vec_key, nv, vecs, vec_id);
+    uint32_t mine[kMaxTop * 32 / kThreads];
+    int nmine = 0;
+#pragma unroll
+    for (int j = 0; j < kMaxTop * 32 / kThreads; ++j) {
+      const int i = tid + j * kThreads;
+      mine[j] = 0xffffffffu;
+      if (i < nv && vec_cut.chosen(s_vec_key[i], vec_id(i))) mine[j] = vec_id(i), ++nmine;
+    }
+    __syncthreads();                                 // s_run is read no more
+#pragma unroll
+    for (int j = 0; j < kMaxTop * 32 / kThreads; ++j)
+      if (mine[j] != 0xffffffffu) s_run[atomicAdd(&s_count, 1)] = mine[j];
+    __syncthreads();
+    if (tid == 0) s_count = 0;
+    __syncthreads();
+    // their values: what is below the worst chosen vector's best cannot be among the best
+    if (tid < vecs * kN) {
+      const int id = static_cast<int>(s_run[tid / kN]) * kN - r.head + tid % kN;
+      if (id >= 0 && id < r.V) {
+        const uint32_t key = order_key(to_float(r.x[id]));
+        if (key >= vec_cut.key) s_cand[atomicAdd(&s_count, 1)] = Entry{key, static_cast<uint32_t>(id)};
+      }
+    }
+    __syncthreads();
+    const int cands = s_count;
+    if (tid < cands) {
+      const Entry e = s_cand[tid];
+      int place = 0;
+      for (int i = 0; i < cands; ++i) place += before(s_cand[i], e);
+      if (place < want) s_best[place] = e;
+    }
+    if (tid == 0) s_nbest = want;
+  }
+  __syncthreads();
+
+  // ---------------------------------------------------------------- the row
+  Sums a = s_part;
+  int nbest = s_nbest;
+  const Entry* best = s_best;
+  if (p.cluster > 1) {
+    cluster_arrive();
+    cluster_wait();
+    if (rank == 0) {
+      // the parts in rank order; every CTA's best ranked among all of them
+      int total = nbest;
+      if (tid < nbest) s_cand[tid] = s_best[tid];
+      for (int c = 1; c < p.cluster; ++c) {
+        auto remote = [&](const void* local) {
+          uint32_t v;
+          asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(mapa_shared(smem_u32(local), c)) : "memory");
+          return v;
+        };
+        const Sums b{__uint_as_float(remote(&s_part.m)), __uint_as_float(remote(&s_part.s)),
+                     __uint_as_float(remote(&s_part.t))};
+        a = join(a, b);
+        if (p.top > 0) {
+          const int nb = static_cast<int>(remote(&s_nbest));
+          if (tid < nb) s_cand[total + tid] = Entry{remote(&s_best[tid].key), remote(&s_best[tid].id)};
+          total += nb;
+        }
+      }
+      __syncthreads();
+      if (tid < total) {
+        const Entry e = s_cand[tid];
+        int place = 0;
+        for (int i = 0; i < total; ++i) place += before(s_cand[i], e);
+        if (place < p.top) s_best[place] = e;
+      }
+      nbest = p.top;
+      __syncthreads();
+    }
+  }
+  if (rank == 0) {
+    // a row that is all -inf has S = 0 and m = -inf: no distribution, NaN throughout
+    const float lse = a.m == -CUDART_INF_F ? CUDART_NAN_F : logf(a.s);
+    if (tid == 0) {
+      p.logprob[row] = (xt - a.m) - lse;
+      p.entropy[row] = lse - a.t / a.s * kLn2;
+    }
+    if (tid < nbest) {
+      const Entry e = best[tid];
+      p.top_ids[row * p.top + tid] = e.id;
+      p.top_logprobs[row * p.top + tid] = (key_value(e.key) - a.m) - lse;
+    }
+  }
+  if (p.cluster > 1) {       // nobody leaves while its part is being read
+    cluster_arrive();
+    cluster_wait();
+  }
+}
+
+template <typename T>
+int run(const Params& p, int64_t M, cudaStream_t stream) {
+  const int64_t row_vectors = (p.V + 2 * Vec<T>::kN - 2) / Vec<T>::kN + 1;       // with any alignment
+  const int64_t segments = (row_vectors + 31) / 32;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(M * p.cluster));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = p.top > 0 ? static_cast<size_t>(segments / p.cluster + 1) * 4 : 0;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = static_cast<unsigned>(p.cluster);
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  LCG_CUDA_OK(cudaLaunchKernelEx(&cfg, k_token_logprobs<T>, p));
+  count_launch();
+  return LCG_OK;
 }
 
 }  // namespace
@@ -112,31 +531,35 @@ extern "C" int lcg_token_logprobs(const void* logits, int dtype, int64_t M, int6
                                   int64_t* top_ids, void* stream) {
   if (!logits || !tokens || !logprob || !entropy || (top > 0 && (!top_logprobs || !top_ids)))
     return fail(LCG_ERR_BAD_ARG, "NULL argument");
-  if (M < 1 || M > 0x7fffffffLL || V < 1 || V > 0x7fffff00LL)
-    return fail(LCG_ERR_UNSUPPORTED_SHAPE, "bad extents M=%lld V=%lld", (long long)M, (long long)V);
+  if (M < 1 || M > 0x7fffffffLL / kMaxCluster || V < 1 || V > kMaxColumns)
+    return fail(LCG_ERR_UNSUPPORTED_SHAPE, "needs 1 <= V <= %lld, got M=%lld V=%lld", (long long)kMaxColumns,
+                (long long)M, (long long)V);
   if (ld < V && M > 1) return fail(LCG_ERR_BAD_ARG, "leading dimension below extent");
   if (token_bytes != 4 && token_bytes != 8) return fail(LCG_ERR_BAD_ARG, "token ids must have 4 or 8 bytes");
   if (top < 0 || top > kMaxTop || top > V)
     return fail(LCG_ERR_BAD_ARG, "top must be between 0 and min(%d, V), got %d", kMaxTop, top);
+  if (dtype != LCG_DTYPE_BF16 && dtype != LCG_DTYPE_FP16 && dtype != LCG_DTYPE_FP32)
+    return fail(LCG_ERR_BAD_ARG, "unknown dtype %d", dtype);
+  const uintptr_t width = dtype == LCG_DTYPE_FP32 ? 4 : 2;
+  if (reinterpret_cast<uintptr_t>(logits) % width != 0)
+    return fail(LCG_ERR_MISALIGNED, "logits must be aligned to their type");
+  Params p;
+  p.logits = logits;
+  p.tokens = tokens;
+  p.ld = ld;
+  p.V = static_cast<int32_t>(V);
+  p.top = top;
+  p.token_bytes = token_bytes;
+  p.logprob = logprob;
+  p.entropy = entropy;
+  p.top_logprobs = top_logprobs;
+  p.top_ids = top_ids;
+  // CTAs to a row: enough to give every SM four CTAs, each with at least 16 segments (two loads a warp).
+  const int64_t segments = (V * static_cast<int64_t>(width) + 511) / 512;
+  p.cluster = 1;
+  while (p.cluster < kMaxCluster && M * p.cluster < 4 * sm_count() && segments / (2 * p.cluster) >= 16) p.cluster *= 2;
   auto st = static_cast<cudaStream_t>(stream);
-  const unsigned grid = static_cast<unsigned>(M);
-  switch (dtype) {
-    case LCG_DTYPE_BF16:
-      k_token_logprobs<<<grid, kThreads, 0, st>>>(static_cast<const __nv_bfloat16*>(logits), V, ld, tokens, token_bytes,
-                                                  top, logprob, entropy, top_logprobs, top_ids);
-      break;
-    case LCG_DTYPE_FP16:
-      k_token_logprobs<<<grid, kThreads, 0, st>>>(static_cast<const __half*>(logits), V, ld, tokens, token_bytes, top,
-                                                  logprob, entropy, top_logprobs, top_ids);
-      break;
-    case LCG_DTYPE_FP32:
-      k_token_logprobs<<<grid, kThreads, 0, st>>>(static_cast<const float*>(logits), V, ld, tokens, token_bytes, top,
-                                                  logprob, entropy, top_logprobs, top_ids);
-      break;
-    default:
-      return fail(LCG_ERR_BAD_ARG, "unknown dtype %d", dtype);
-  }
-  LCG_CUDA_OK(cudaGetLastError());
-  count_launch();
-  return LCG_OK;
+  if (dtype == LCG_DTYPE_BF16) return run<__nv_bfloat16>(p, M, st);
+  if (dtype == LCG_DTYPE_FP16) return run<__half>(p, M, st);
+  return run<float>(p, M, st);
 }

@@ -603,7 +603,7 @@ _LOGIT_TYPES = {BF16: nat.DTYPE_BF16, torch.float16: nat.DTYPE_FP16, torch.float
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> TokenLogprobs:
     """Log probability of ``tokens[i]`` under ``softmax(logits[i])``, each row's entropy, and its ``top``
     (0 to 32) most likely tokens, in one pass over ``logits (M, V)`` (bf16, fp16 or fp32, unit stride along
-    V).  ``-inf`` masks a token.  A row that is all ``-inf``, or holds ``+inf`` or a NaN, gives NaN; an id
+    V, V at most 2^20).  ``-inf`` masks a token.  A row that is all ``-inf``, or holds ``+inf`` or a NaN, gives NaN; an id
     outside ``[0, V)`` gives a NaN log probability for its row."""
     for t, what in ((logits, "logits"), (tokens, "tokens")):
         if not isinstance(t, torch.Tensor) or not t.is_cuda:
