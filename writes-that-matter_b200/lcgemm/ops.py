@@ -7,14 +7,13 @@ also fp16 and fp32 logits); there is no CPU implementation behind these calls.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 from typing import NamedTuple
 
 import torch
 
 from . import _native as nat
-from ._native import NativeScheme, check, lib, ptr, stream_ptr
+from ._native import NativeScheme, check, lib, ptr, raw_stream, stream_ptr
 
 BF16 = torch.bfloat16
 E4M3 = torch.float8_e4m3fn
@@ -456,24 +455,35 @@ def add(a: torch.Tensor, b: torch.Tensor, out: torch.Tensor | None = None) -> to
 
 
 # ------------------------------------------- 8-bit operands, a scale per 128
-def _on(t: torch.Tensor, *others):
-    """Context in which ``t``'s device is current; every tensor of a call lives there."""
-    for o in others:
-        if o is not None and o.device != t.device:
-            raise ValueError(f"all tensors of a call must be on one device, got {t.device} and {o.device}")
-    if t.device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(t.device)
+# One call of these on a single token is shorter on the GPU than on the host, so the host side is kept
+# short: one allocation call per output, the raw stream handle, no context managers on the usual path.
+_current_device = torch.cuda.current_device
+_empty = torch.empty_strided
+_F32 = torch.float32
+
+
+def _need_here(dev: int, *tensors) -> None:
+    for t in tensors:
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"all tensors of a call must be on one device, got cuda:{dev} and {t.device}")
+
+
+def _need_cuda(t, what: str) -> None:
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise RuntimeError(
+            f"{what} must be a CUDA tensor: lcgemm_b200 has no CPU implementation of this path")
 
 
 def _codes(m: int, k: int, device):
     """An (m, k) view of codes whose row pitch is a multiple of 16 bytes."""
+    if k % 16 == 0:
+        return _empty((m, k), (k, 1), dtype=E4M3, device=device)
     return torch.empty((m, (k + 15) // 16 * 16), dtype=E4M3, device=device)[:, :k]
 
 
 def _row_scales(m: int, k: int, device):
     """(m, blocks) scales with the rows contiguous: the order the product reads fastest."""
-    return torch.empty((-(-k // FP8_BLOCK), m), dtype=torch.float32, device=device).t()
+    return _empty((m, -(-k // FP8_BLOCK)), (1, max(m, 1)), dtype=_F32, device=device)
 
 
 def quantize_fp8(x: torch.Tensor, block_rows: int = 1):
@@ -490,15 +500,20 @@ def quantize_fp8(x: torch.Tensor, block_rows: int = 1):
     m, k = x.shape
     if k < 1:
         raise ValueError("x has no columns")
-    with _on(x):
-        q = _codes(m, k, x.device)
-        if block_rows == 1:
-            scale = _row_scales(m, k, x.device)
-        else:
-            scale = torch.empty((-(-m // FP8_BLOCK), -(-k // FP8_BLOCK)), dtype=torch.float32, device=x.device)
-        if m > 0:
-            check(lib().lcg_quantize_fp8(ptr(x), m, k, x.stride(0), block_rows, ptr(q), q.stride(0), ptr(scale),
-                                         scale.stride(0), scale.stride(1), stream_ptr()))
+    dev = x.get_device()
+    if dev != _current_device():
+        with torch.cuda.device(dev):
+            return quantize_fp8(x, block_rows)
+    device = x.device
+    q = _codes(m, k, device)
+    if block_rows == 1:
+        scale = _row_scales(m, k, device)
+    else:
+        scale = torch.empty((-(-m // FP8_BLOCK), -(-k // FP8_BLOCK)), dtype=_F32, device=device)
+    if m > 0:
+        s_row, s_blk = scale.stride()
+        check(lib().lcg_quantize_fp8(x.data_ptr(), m, k, x.stride(0), block_rows, q.data_ptr(), q.stride(0),
+                                     scale.data_ptr(), s_row, s_blk, raw_stream(dev)))
     return q, scale
 
 
@@ -506,30 +521,38 @@ def add_rmsnorm_fp8(delta, residual, norm_weight, eps: float, residual_out=None)
     """:func:`add_rmsnorm` with an 8-bit result: ``(codes, scales, delta + residual)``, the norm
     quantised by rows from its fp32 value.  Without a ``delta`` the third value is ``residual`` itself
     and nothing is stored for it.  ``residual_out`` may be ``residual``."""
-    tensors = [(residual, "residual"), (norm_weight, "norm weight")]
-    if delta is not None:
-        tensors.append((delta, "delta"))
-        if residual_out is not None:
-            tensors.append((residual_out, "residual_out"))
-    for t, what in tensors:
-        _need(t, what)
-    if residual.dim() != 2:
-        raise ValueError(f"residual must be a matrix, got {tuple(residual.shape)}")
-    m, k = residual.shape
-    for t, what in tensors:
-        want = (k,) if t is norm_weight else (m, k)
-        if tuple(t.shape) != want or not t.is_contiguous():
-            raise ValueError(f"{what} must be a contiguous {want} tensor")
-    with _on(residual, norm_weight, delta, residual_out):
-        if delta is None:
-            residual_out = None
-        elif residual_out is None:
+    _need(residual, "residual"), _need(norm_weight, "norm weight")
+    if residual.dim() != 2 or not residual.is_contiguous():
+        raise ValueError(f"residual must be a contiguous matrix, got {tuple(residual.shape)}")
+    shape = residual.shape
+    m, k = shape
+    if norm_weight.shape != (k,) or not norm_weight.is_contiguous():
+        raise ValueError(f"norm weight must be a contiguous ({k},) tensor")
+    if delta is None:
+        residual_out = None
+    else:
+        for t, what in ((delta, "delta"), (residual_out, "residual_out")):
+            if t is not None:
+                _need(t, what)
+                if t.shape != shape or not t.is_contiguous():
+                    raise ValueError(f"{what} must be a contiguous ({m}, {k}) tensor")
+    dev = residual.get_device()
+    _need_here(dev, norm_weight, delta, residual_out)
+    if dev != _current_device():
+        with torch.cuda.device(dev):
+            return add_rmsnorm_fp8(delta, residual, norm_weight, eps, residual_out)
+    if delta is None:
+        d_ptr = h_ptr = None
+    else:
+        if residual_out is None:
             residual_out = torch.empty_like(residual)
-        q, scale = _codes(m, k, residual.device), _row_scales(m, k, residual.device)
-        if m > 0:
-            check(lib().lcg_add_rmsnorm_fp8(None if delta is None else ptr(delta), ptr(residual), ptr(norm_weight), m, k,
-                                            float(eps), None if delta is None else ptr(residual_out), ptr(q),
-                                            q.stride(0), ptr(scale), scale.stride(0), scale.stride(1), stream_ptr()))
+        d_ptr, h_ptr = delta.data_ptr(), residual_out.data_ptr()
+    device = residual.device
+    q, scale = _codes(m, k, device), _row_scales(m, k, device)
+    if m > 0:
+        s_row, s_blk = scale.stride()
+        check(lib().lcg_add_rmsnorm_fp8(d_ptr, residual.data_ptr(), norm_weight.data_ptr(), m, k, eps, h_ptr,
+                                        q.data_ptr(), q.stride(0), scale.data_ptr(), s_row, s_blk, raw_stream(dev)))
     return q, scale, residual if delta is None else residual_out
 
 
@@ -539,11 +562,16 @@ def swiglu_fp8(z: torch.Tensor):
     if z.dim() != 2 or z.shape[1] % 2 != 0:
         raise ValueError(f"z must be an (M, 2 * I) matrix, got {tuple(z.shape)}")
     m, inter = z.shape[0], z.shape[1] // 2
-    with _on(z):
-        q, scale = _codes(m, inter, z.device), _row_scales(m, inter, z.device)
-        if m > 0:
-            check(lib().lcg_swiglu_fp8(ptr(z), m, inter, z.stride(0), ptr(q), q.stride(0), ptr(scale),
-                                       scale.stride(0), scale.stride(1), stream_ptr()))
+    dev = z.get_device()
+    if dev != _current_device():
+        with torch.cuda.device(dev):
+            return swiglu_fp8(z)
+    device = z.device
+    q, scale = _codes(m, inter, device), _row_scales(m, inter, device)
+    if m > 0:
+        s_row, s_blk = scale.stride()
+        check(lib().lcg_swiglu_fp8(z.data_ptr(), m, inter, z.stride(0), q.data_ptr(), q.stride(0), scale.data_ptr(),
+                                   s_row, s_blk, raw_stream(dev)))
     return q, scale
 
 
@@ -554,37 +582,41 @@ def gemm_fp8(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: t
     quantisers' are the fastest).  Codes have unit stride along K and a row pitch of a multiple of 16
     bytes, as the quantisers return them.  Each block's sum and the scaled sum are fp32."""
     for t, what in ((a, "a"), (b, "b"), (a_scale, "a_scale"), (b_scale, "b_scale")):
-        if not isinstance(t, torch.Tensor) or not t.is_cuda:
-            raise RuntimeError(
-                f"{what} must be a CUDA tensor: lcgemm_b200 has no CPU implementation of this path")
+        _need_cuda(t, what)
         if t.dim() != 2:
             raise ValueError(f"{what} must be a matrix, got {tuple(t.shape)}")
     if a.dtype != E4M3 or b.dtype != E4M3:
         raise ValueError(f"a and b must be float8_e4m3fn, got {a.dtype} and {b.dtype}")
-    if a_scale.dtype != torch.float32 or b_scale.dtype != torch.float32:
+    if a_scale.dtype != _F32 or b_scale.dtype != _F32:
         raise ValueError(f"scales must be float32, got {a_scale.dtype} and {b_scale.dtype}")
     (m, k), (n, kb) = a.shape, b.shape
     if kb != k:
         raise ValueError(f"inner dimensions differ: {k} vs {kb}")
     if k < 1 or n < 1:
         raise ValueError(f"empty product: N={n}, K={k}")
-    if (a.stride(1) != 1 or b.stride(1) != 1) and k > 1:
+    (lda, ka), (ldb, kb) = a.stride(), b.stride()
+    if (ka != 1 or kb != 1) and k > 1:
         raise ValueError("codes must be row-major (unit stride along their last dimension)")
-    blocks = -(-k // FP8_BLOCK)
-    if tuple(a_scale.shape) != (m, blocks) or tuple(b_scale.shape) != (-(-n // FP8_BLOCK), blocks):
-        raise ValueError(f"scales must be {(m, blocks)} and {(-(-n // FP8_BLOCK), blocks)}, got "
+    blocks, rows = -(-k // FP8_BLOCK), -(-n // FP8_BLOCK)
+    if a_scale.shape != (m, blocks) or b_scale.shape != (rows, blocks):
+        raise ValueError(f"scales must be {(m, blocks)} and {(rows, blocks)}, got "
                          f"{tuple(a_scale.shape)} and {tuple(b_scale.shape)}")
     if out is not None:
         _need(out, "out")
-        if tuple(out.shape) != (m, n):
+        if out.shape != (m, n):
             raise ValueError(f"out must be ({m}, {n}), got {tuple(out.shape)}")
-    with _on(a, b, a_scale, b_scale, out):
-        if out is None:
-            out = _padded_out(m, n, a.device)
-        if m > 0:
-            check(lib().lcg_gemm_fp8(ptr(a), a.stride(0), ptr(a_scale), a_scale.stride(0), a_scale.stride(1),
-                                     ptr(b), b.stride(0), ptr(b_scale), b_scale.stride(0), b_scale.stride(1),
-                                     ptr(out), out.stride(0), m, n, k, ptr(status_word(a.device)), stream_ptr()))
+    dev = a.get_device()
+    _need_here(dev, b, a_scale, b_scale, out)
+    if dev != _current_device():
+        with torch.cuda.device(dev):
+            return gemm_fp8(a, a_scale, b, b_scale, out)
+    if out is None:
+        out = _empty((m, n), (n, 1), dtype=BF16, device=a.device) if n % 8 == 0 else _padded_out(m, n, a.device)
+    if m > 0:
+        (as_row, as_blk), (bs_row, bs_blk) = a_scale.stride(), b_scale.stride()
+        check(lib().lcg_gemm_fp8(a.data_ptr(), lda, a_scale.data_ptr(), as_row, as_blk, b.data_ptr(), ldb,
+                                 b_scale.data_ptr(), bs_row, bs_blk, out.data_ptr(), out.stride(0), m, n, k,
+                                 status_word(a.device).data_ptr(), raw_stream(dev)))
     return out
 
 
@@ -603,31 +635,34 @@ _LOGIT_TYPES = {BF16: nat.DTYPE_BF16, torch.float16: nat.DTYPE_FP16, torch.float
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> TokenLogprobs:
     """Log probability of ``tokens[i]`` under ``softmax(logits[i])``, each row's entropy, and its ``top``
     (0 to 32) most likely tokens, in one pass over ``logits (M, V)`` (bf16, fp16 or fp32, unit stride along
-    V, V at most 2^20).  ``-inf`` masks a token.  A row that is all ``-inf``, or holds ``+inf`` or a NaN, gives NaN; an id
-    outside ``[0, V)`` gives a NaN log probability for its row."""
-    for t, what in ((logits, "logits"), (tokens, "tokens")):
-        if not isinstance(t, torch.Tensor) or not t.is_cuda:
-            raise RuntimeError(
-                f"{what} must be a CUDA tensor: lcgemm_b200 has no CPU implementation of this path")
+    V, V at most 2^20).  ``-inf`` masks a token.  A row that is all ``-inf``, or holds ``+inf`` or a NaN, gives
+    NaN; an id outside ``[0, V)`` gives a NaN log probability for its row."""
+    _need_cuda(logits, "logits"), _need_cuda(tokens, "tokens")
     kind = _LOGIT_TYPES.get(logits.dtype)
     if kind is None:
         raise ValueError(f"logits must be bfloat16, float16 or float32, got {logits.dtype}")
     if logits.dim() != 2 or (logits.stride(1) != 1 and logits.shape[1] > 1):
         raise ValueError(f"logits must be a row-major (M, V) matrix, got {tuple(logits.shape)}")
     m, v = logits.shape
-    if tokens.dtype not in (torch.int64, torch.int32) or tuple(tokens.shape) != (m,):
+    if tokens.dtype not in (torch.int64, torch.int32) or tokens.shape != (m,):
         raise ValueError(f"tokens must be ({m},) of int64 or int32, got {tuple(tokens.shape)} of {tokens.dtype}")
-    if not 0 <= top <= min(MAX_TOP, v):
-        raise ValueError(f"top must be between 0 and {min(MAX_TOP, v)}, got {top}")
     if v < 1:
         raise ValueError("logits have no columns")
-    with _on(logits, tokens):
-        tokens = tokens.contiguous()
-        dev = logits.device
-        logprob, entropy = torch.empty((2, m), dtype=torch.float32, device=dev).unbind(0)
-        top_lp = torch.empty((m, top), dtype=torch.float32, device=dev)
-        top_ids = torch.empty((m, top), dtype=torch.int64, device=dev)
-        if m > 0:
-            check(lib().lcg_token_logprobs(ptr(logits), kind, m, v, logits.stride(0), ptr(tokens), tokens.element_size(),
-                                           top, ptr(logprob), ptr(entropy), ptr(top_lp), ptr(top_ids), stream_ptr()))
+    if not 0 <= top <= min(MAX_TOP, v):
+        raise ValueError(f"top must be between 0 and {min(MAX_TOP, v)}, got {top}")
+    dev = logits.get_device()
+    _need_here(dev, tokens)
+    if dev != _current_device():
+        with torch.cuda.device(dev):
+            return token_logprobs(logits, tokens, top)
+    tokens = tokens.contiguous()
+    device = logits.device
+    logprob, entropy = _empty((m,), (1,), dtype=_F32, device=device), _empty((m,), (1,), dtype=_F32, device=device)
+    pitch = max(top, 1)
+    top_lp = _empty((m, top), (pitch, 1), dtype=_F32, device=device)
+    top_ids = _empty((m, top), (pitch, 1), dtype=torch.int64, device=device)
+    if m > 0:
+        check(lib().lcg_token_logprobs(logits.data_ptr(), kind, m, v, logits.stride(0), tokens.data_ptr(),
+                                       tokens.element_size(), top, logprob.data_ptr(), entropy.data_ptr(),
+                                       top_lp.data_ptr(), top_ids.data_ptr(), raw_stream(dev)))
     return TokenLogprobs(logprob, entropy, top_lp, top_ids)
