@@ -9,9 +9,12 @@
 // leaves each segment's maximum in shared memory.  Of any partition into runs of consecutive ids, the
 // `top` best values (larger first, lower id first among equals) lie in the `top` best runs by the
 // same order of their maxima: a run outside has `top` runs before it, each with a value that comes
-// before all of its own.  So the `top` best segments are read again, of those the `top` best vectors are
-// kept, and of their at most 256 values each is ranked by counting.  The cost does not depend on the
-// values: no order of the row and no number of ties makes it longer.
+// before all of its own.  So the `top` best segments are read again, and the values in them that are
+// not below the worst of those segments' maxima, seldom more than two or three times `top`, are each
+// ranked by counting.  Where they are more than 256 (long ties, rising rows), the same rule is applied
+// once more, to the vectors of those segments: at most 32 x 8 values are then left, whatever the row
+// holds.  (The second rule for every row, with its threshold searched by the whole CTA, took longer than
+// the pass: 436 us against 199 for 4096 rows of 151936 bf16 without alternatives.)
 //
 // Bound by HBM for many rows (2 or 4 bytes a value; the exponential unit is at 3/4 of its rate on bf16), by the
 // latency of the selection for one row.  A row is one CTA's, or a cluster's of up to eight when there
@@ -31,6 +34,7 @@ constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxTop = 32;
 constexpr int kMaxCluster = 8;
+constexpr int kMaxCands = kMaxCluster * kMaxTop;      // = 32 vectors of 8 values
 constexpr int64_t kMaxColumns = 1 << 20;     // a row's segment maxima then take at most 32 KiB
 constexpr int kUnroll = 4;                   // 16-byte loads of a thread in flight
 
@@ -125,15 +129,27 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
 }
 
 // Order of the alternatives as whole numbers: larger is better, 0 and -0 alike, NaN with -inf; 0 is
-// no value's.
+// no value's.  The low bits that T's values leave alike are dropped: fewer bits to search.
+template <typename T>
+struct Key;
+template <>
+struct Key<float> { static constexpr int kLow = 0; };
+template <>
+struct Key<__nv_bfloat16> { static constexpr int kLow = 16; };
+template <>
+struct Key<__half> { static constexpr int kLow = 13; };
+template <typename T>
 __device__ __forceinline__ uint32_t order_key(float v) {
   v = v + 0.0f;
   if (v != v) v = -CUDART_INF_F;
   const uint32_t b = __float_as_uint(v);
-  return (b & 0x80000000u) ? ~b : b | 0x80000000u;
+  return ((b & 0x80000000u) ? ~b : b | 0x80000000u) >> Key<T>::kLow;
 }
+template <typename T>
 __device__ __forceinline__ float key_value(uint32_t key) {
-  return __uint_as_float((key & 0x80000000u) ? key & 0x7fffffffu : ~key);
+  constexpr int kLow = Key<T>::kLow;
+  const uint32_t full = key << kLow;
+  return __uint_as_float((full & 0x80000000u) ? full & 0x7fffffffu : ~(full | ((1u << kLow) - 1u)));
 }
 
 // A running maximum with the sums that go with it; T in units of ln 2, as the exponentials are taken
@@ -200,39 +216,55 @@ struct Row {
 };
 
 // The k-th best of keys[0, n) (n >= k), and among values equal to it the ids below `limit` are in:
-// then exactly k of the keys satisfy chosen().  id_of gives the ids, which differ.  All threads call it.
+// then exactly k of the keys satisfy chosen().  id_of gives the ids, which differ.  `count` counts the
+// indexes that satisfy a predicate; it is the same for all threads that take part.
 struct Cut {
   uint32_t key, limit;
   __device__ bool chosen(uint32_t k, uint32_t id) const { return k > key || (k == key && id < limit); }
 };
-template <typename IdOf>
-__device__ Cut find_cut(const uint32_t* keys, int n, int k, IdOf id_of) {
-  auto count = [&](auto pred) {
+template <int kBits, typename Count, typename IdOf>
+__device__ __forceinline__ Cut find_cut(const uint32_t* keys, int n, int k, Count count, IdOf id_of) {
+  Cut cut{0u, 0xffffffffu};
+  if (n == k) return cut;
+  for (int b = kBits - 1; b >= 0; --b) {
+    const uint32_t cand = cut.key | (1u << b);
+    const int c = count([&](int i) { return keys[i] >= cand; });
+    if (c >= k) cut.key = cand;
+    if (c == k) return cut;
+  }
+  const int better = count([&](int i) { return keys[i] > cut.key; });
+  uint32_t limit = 0;               // the largest limit that lets no more than k in
+  for (int b = 30; b >= 0; --b) {
+    const uint32_t cand = limit | (1u << b);
+    const int in = count([&](int i) { return keys[i] == cut.key && static_cast<uint32_t>(id_of(i)) < cand; });
+    if (better + in <= k) limit = cand;
+  }
+  cut.limit = limit;
+  return cut;
+}
+// Counting by one warp and by the whole CTA.
+struct WarpCount {
+  int n;
+  template <typename Pred>
+  __device__ __forceinline__ int operator()(Pred pred) const {
+    int c = 0;
+#pragma unroll 4
+    for (int i = threadIdx.x & 31; i < n; i += 32) c += pred(i);
+    return __reduce_add_sync(0xffffffffu, c);
+  }
+};
+struct CtaCount {
+  int n;
+  template <typename Pred>
+  __device__ __forceinline__ int operator()(Pred pred) const {
     int c = 0;
     for (int i0 = 0; i0 < n; i0 += kThreads) {
       const int i = i0 + static_cast<int>(threadIdx.x);
-      c += __syncthreads_count(i < n && pred(keys[i < n ? i : 0], i));
+      c += __syncthreads_count(i < n && pred(i));
     }
     return c;
-  };
-  Cut cut{0u, 0xffffffffu};
-  for (int b = 31; b >= 0; --b) {
-    const uint32_t cand = cut.key | (1u << b);
-    if (count([&](uint32_t key, int) { return key >= cand; }) >= k) cut.key = cand;
   }
-  const int better = count([&](uint32_t key, int) { return key > cut.key; });
-  const int ties = count([&](uint32_t key, int) { return key == cut.key; });
-  if (better + ties > k) {        // the largest limit that lets no more than k in
-    uint32_t limit = 0;
-    for (int b = 30; b >= 0; --b) {
-      const uint32_t cand = limit | (1u << b);
-      const int in = count([&](uint32_t key, int i) { return key == cut.key && static_cast<uint32_t>(id_of(i)) < cand; });
-      if (better + in <= k) limit = cand;
-    }
-    cut.limit = limit;
-  }
-  return cut;
-}
+};
 
 struct Entry {
   uint32_t key, id;
@@ -250,6 +282,8 @@ struct Params {
   int64_t* top_ids;
 };
 
+static_assert(kMaxCluster <= kWarps && kMaxTop <= 32 && kMaxCands == kThreads, "a warp to a CTA's part, a lane to an entry");
+
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 5)
 k_token_logprobs(const __grid_constant__ Params p) {
@@ -261,7 +295,8 @@ k_token_logprobs(const __grid_constant__ Params p) {
   __shared__ int s_nbest;
   __shared__ uint32_t s_run[kMaxTop];              // chosen segments, then chosen vectors
   __shared__ uint32_t s_vec_key[kMaxTop * 32];
-  __shared__ Entry s_cand[kMaxCluster * kMaxTop];
+  __shared__ Entry s_cand[kMaxCands];
+  __shared__ Cut s_cut;
   __shared__ int s_count;
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -293,7 +328,7 @@ k_token_logprobs(const __grid_constant__ Params p) {
     if (p.top > 0 && lane == 0) {
 #pragma unroll
       for (int u = 0; u < kUnroll; ++u)
-        if (u < count) s_keys[seg + u * kWarps - seg0] = order_key(mx[u]);
+        if (u < count) s_keys[seg + u * kWarps - seg0] = order_key<T>(mx[u]);
     }
     float grown = m;
 #pragma unroll
@@ -384,55 +419,81 @@ k_token_logprobs(const __grid_constant__ Params p) {
   if (want > 0) {
     const int n = seg1 - seg0;
     const int runs = min(want, n);
-    const Cut seg_cut = find_cut(s_keys, n, runs, [&](int i) { return i; });
-    for (int i = tid; i < n; i += kThreads)
-      if (seg_cut.chosen(s_keys[i], i)) s_run[atomicAdd(&s_count, 1)] = seg0 + i;
+    constexpr int kBits = 32 - Key<T>::kLow;
+    auto itself = [](int i) { return i; };
+    if (warp == 0) {
+      const Cut cut = find_cut<kBits>(s_keys, n, runs, WarpCount{n}, itself);
+      int at = 0;
+      for (int i0 = 0; i0 < n; i0 += 32) {
+        const int i = i0 + lane;
+        const uint32_t in = __ballot_sync(0xffffffffu, i < n && cut.chosen(s_keys[i < n ? i : 0], i));
+        if (in & (1u << lane)) s_run[at + __popc(in & ((1u << lane) - 1u))] = seg0 + i;
+        at += __popc(in);
+      }
+      if (lane == 0) s_cut = cut;
+    }
     __syncthreads();
-    // every vector of the chosen segments: its best value, 0 where it holds none of the row
-    const int nv = runs * 32;
-    for (int i = tid; i < nv; i += kThreads) {
-      const int v = static_cast<int>(s_run[i >> 5]) * 32 + (i & 31);
-      uint32_t key = 0;
+    // No value below the least of the chosen maxima is among the best: there are `runs` that are not.
+    // (Where all segments are chosen there is no such bound.)
+    const uint32_t least = n > want ? s_cut.key : 0u;
+    for (int j = warp; j < runs; j += kWarps) {
+      const int v = static_cast<int>(s_run[j]) * 32 + lane;
       if (v < nvec) {
         float f[kN];
         Vec<T>::unpack(r.load(v), f);
 #pragma unroll
         for (int e = 0; e < kN; ++e) {
           const int id = v * kN - r.head + e;
-          if (id >= 0 && id < r.V) key = max(key, order_key(f[e]));
+          const uint32_t key = order_key<T>(f[e]);
+          if (key >= least && id >= 0 && id < r.V) {
+            const int at = atomicAdd(&s_count, 1);
+            if (at < kMaxCands) s_cand[at] = Entry{key, static_cast<uint32_t>(id)};
+          }
         }
       }
-      s_vec_key[i] = key;
     }
-    if (tid == 0) s_count = 0;
     __syncthreads();
-    const int vecs = min(want, nv);
-    auto vec_id = [&](int i) { return static_cast<int>(s_run[i >> 5]) * 32 + (i & 31); };
-    const Cut vec_cut = find_cut(s_vec_key, nv, vecs, vec_id);
-    uint32_t mine[kMaxTop * 32 / kThreads];
-    int nmine = 0;
+    if (s_count > kMaxCands) {
+      // Too many: the best vectors of these segments, each by its best value (0 where it holds none of the row).
+      const int nv = runs * 32;
+      for (int i = tid; i < nv; i += kThreads) {
+        const int v = static_cast<int>(s_run[i >> 5]) * 32 + (i & 31);
+        uint32_t key = 0;
+        if (v < nvec) {
+          float f[kN];
+          Vec<T>::unpack(r.load(v), f);
 #pragma unroll
-    for (int j = 0; j < kMaxTop * 32 / kThreads; ++j) {
-      const int i = tid + j * kThreads;
-      mine[j] = 0xffffffffu;
-      if (i < nv && vec_cut.chosen(s_vec_key[i], vec_id(i))) mine[j] = vec_id(i), ++nmine;
-    }
-    __syncthreads();                                 // s_run is read no more
-#pragma unroll
-    for (int j = 0; j < kMaxTop * 32 / kThreads; ++j)
-      if (mine[j] != 0xffffffffu) s_run[atomicAdd(&s_count, 1)] = mine[j];
-    __syncthreads();
-    if (tid == 0) s_count = 0;
-    __syncthreads();
-    // their values: what is below the worst chosen vector's best cannot be among the best
-    if (tid < vecs * kN) {
-      const int id = static_cast<int>(s_run[tid / kN]) * kN - r.head + tid % kN;
-      if (id >= 0 && id < r.V) {
-        const uint32_t key = order_key(to_float(r.x[id]));
-        if (key >= vec_cut.key) s_cand[atomicAdd(&s_count, 1)] = Entry{key, static_cast<uint32_t>(id)};
+          for (int e = 0; e < kN; ++e) {
+            const int id = v * kN - r.head + e;
+            if (id >= 0 && id < r.V) key = max(key, order_key<T>(f[e]));
+          }
+        }
+        s_vec_key[i] = key;
       }
+      __syncthreads();
+      if (tid == 0) s_count = 0;
+      const int vecs = min(want, nv);
+      auto vec_id = [&](int i) { return static_cast<int>(s_run[i >> 5]) * 32 + (i & 31); };
+      const Cut cut = find_cut<kBits>(s_vec_key, nv, vecs, CtaCount{nv}, vec_id);
+      uint32_t mine[kMaxTop * 32 / kThreads];
+#pragma unroll
+      for (int j = 0; j < kMaxTop * 32 / kThreads; ++j) {
+        const int i = tid + j * kThreads;
+        mine[j] = i < nv && cut.chosen(s_vec_key[i], vec_id(i)) ? vec_id(i) : 0xffffffffu;
+      }
+      __syncthreads();                                 // s_run is read no more
+#pragma unroll
+      for (int j = 0; j < kMaxTop * 32 / kThreads; ++j)
+        if (mine[j] != 0xffffffffu) s_run[atomicAdd(&s_count, 1)] = mine[j];
+      __syncthreads();
+      if (tid == 0) s_count = 0;
+      __syncthreads();
+      if (tid < vecs * kN) {
+        const int id = static_cast<int>(s_run[tid / kN]) * kN - r.head + tid % kN;
+        if (id >= 0 && id < r.V) s_cand[atomicAdd(&s_count, 1)] = Entry{order_key<T>(to_float(r.x[id])), static_cast<uint32_t>(id)};
+      }
+      __syncthreads();
     }
-    __syncthreads();
     const int cands = s_count;
     if (tid < cands) {
       const Entry e = s_cand[tid];
@@ -452,26 +513,28 @@ k_token_logprobs(const __grid_constant__ Params p) {
     cluster_arrive();
     cluster_wait();
     if (rank == 0) {
-      // the parts in rank order; every CTA's best ranked among all of them
-      int total = nbest;
-      if (tid < nbest) s_cand[tid] = s_best[tid];
-      for (int c = 1; c < p.cluster; ++c) {
-        auto remote = [&](const void* local) {
-          uint32_t v;
-          asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(mapa_shared(smem_u32(local), c)) : "memory");
-          return v;
-        };
-        const Sums b{__uint_as_float(remote(&s_part.m)), __uint_as_float(remote(&s_part.s)),
-                     __uint_as_float(remote(&s_part.t))};
-        a = join(a, b);
+      // a warp for each CTA's part: its sums and its best, all at once; then ranked among all of them
+      auto remote = [&](const void* local) {
+        uint32_t v;
+        asm volatile("ld.shared::cluster.u32 %0, [%1];"
+                     : "=r"(v) : "r"(mapa_shared(smem_u32(local), static_cast<uint32_t>(warp))) : "memory");
+        return v;
+      };
+      if (warp < p.cluster) {
+        if (lane == 0)
+          s_sums[warp] = Sums{__uint_as_float(remote(&s_part.m)), __uint_as_float(remote(&s_part.s)),
+                              __uint_as_float(remote(&s_part.t))};
         if (p.top > 0) {
           const int nb = static_cast<int>(remote(&s_nbest));
-          if (tid < nb) s_cand[total + tid] = Entry{remote(&s_best[tid].key), remote(&s_best[tid].id)};
-          total += nb;
+          // (this CTA's own list is read from its place too: s_cand is another array)
+          s_cand[tid] = lane < nb ? Entry{remote(&s_best[lane].key), remote(&s_best[lane].id)} : Entry{0u, 0xffffffffu};
         }
       }
       __syncthreads();
-      if (tid < total) {
+      a = s_sums[0];
+      for (int c = 1; c < p.cluster; ++c) a = join(a, s_sums[c]);      // in rank order
+      const int total = p.top > 0 ? p.cluster * kMaxTop : 0;
+      if (tid < total && s_cand[tid].key != 0u) {
         const Entry e = s_cand[tid];
         int place = 0;
         for (int i = 0; i < total; ++i) place += before(s_cand[i], e);
@@ -491,7 +554,7 @@ k_token_logprobs(const __grid_constant__ Params p) {
     if (tid < nbest) {
       const Entry e = best[tid];
       p.top_ids[row * p.top + tid] = e.id;
-      p.top_logprobs[row * p.top + tid] = (key_value(e.key) - a.m) - lse;
+      p.top_logprobs[row * p.top + tid] = (key_value<T>(e.key) - a.m) - lse;
     }
   }
   if (p.cluster > 1) {       // nobody leaves while its part is being read
