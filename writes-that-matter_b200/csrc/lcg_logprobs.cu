@@ -215,56 +215,48 @@ struct Row {
   }
 };
 
-// The k-th best of keys[0, n) (n >= k), and among values equal to it the ids below `limit` are in:
-// then exactly k of the keys satisfy chosen().  id_of gives the ids, which differ.  `count` counts the
-// indexes that satisfy a predicate; it is the same for all threads that take part.
-struct Cut {
-  uint32_t key, limit;
-  __device__ bool chosen(uint32_t k, uint32_t id) const { return k > key || (k == key && id < limit); }
-};
-template <int kBits, typename Count, typename IdOf>
-__device__ __forceinline__ Cut find_cut(const uint32_t* keys, int n, int k, Count count, IdOf id_of) {
-  Cut cut{0u, 0xffffffffu};
-  if (n == k) return cut;
-  for (int b = kBits - 1; b >= 0; --b) {
-    const uint32_t cand = cut.key | (1u << b);
-    const int c = count([&](int i) { return keys[i] >= cand; });
-    if (c >= k) cut.key = cand;
-    if (c == k) return cut;
+// The indexes of the k best of keys[0, n), n >= k, equal ones by rising index, written to `out` in
+// rising order; one warp.  keys is 16-byte aligned, padded with zeros to a multiple of four.  Returns
+// the least of the chosen keys (0 when all are).  The threshold is searched bit by bit from the top and most
+// often found, as the first one that exactly k keys reach, long before the last bit.
+template <int kBits>
+__device__ uint32_t warp_select(const uint32_t* keys, int n, int k, uint32_t* out) {
+  const int lane = threadIdx.x & 31;
+  auto count = [&](uint32_t least) {
+    int c = 0;
+#pragma unroll 5
+    for (int i = lane; i < (n + 3) / 4; i += 32) {
+      const uint4 q = reinterpret_cast<const uint4*>(keys)[i];
+      c += (q.x >= least) + (q.y >= least) + (q.z >= least) + (q.w >= least);
+    }
+    return __reduce_add_sync(0xffffffffu, c);
+  };
+  uint32_t cut = 0;
+  int ties = n;                        // how many keys equal to the cut are taken
+  if (n > k) {
+    bool exact = false;
+    for (int b = kBits - 1; b >= 0 && !exact; --b) {
+      const uint32_t cand = cut | (1u << b);
+      const int c = count(cand);
+      if (c >= k) cut = cand;
+      exact = c == k;
+    }
+    if (!exact) ties = k - count(cut + 1u);
   }
-  const int better = count([&](int i) { return keys[i] > cut.key; });
-  uint32_t limit = 0;               // the largest limit that lets no more than k in
-  for (int b = 30; b >= 0; --b) {
-    const uint32_t cand = limit | (1u << b);
-    const int in = count([&](int i) { return keys[i] == cut.key && static_cast<uint32_t>(id_of(i)) < cand; });
-    if (better + in <= k) limit = cand;
+  int at = 0;
+  for (int i0 = 0; i0 < n; i0 += 32) {
+    const int i = i0 + lane;
+    const uint32_t key = i < n ? keys[i] : 0u;
+    const uint32_t below = (1u << lane) - 1u;
+    const uint32_t equal = __ballot_sync(0xffffffffu, i < n && key == cut);
+    const bool in = i < n && (key > cut || (key == cut && __popc(equal & below) < ties));
+    const uint32_t ins = __ballot_sync(0xffffffffu, in);
+    if (in) out[at + __popc(ins & below)] = i;
+    at += __popc(ins);
+    ties = max(0, ties - __popc(equal));
   }
-  cut.limit = limit;
   return cut;
 }
-// Counting by one warp and by the whole CTA.
-struct WarpCount {
-  int n;
-  template <typename Pred>
-  __device__ __forceinline__ int operator()(Pred pred) const {
-    int c = 0;
-#pragma unroll 4
-    for (int i = threadIdx.x & 31; i < n; i += 32) c += pred(i);
-    return __reduce_add_sync(0xffffffffu, c);
-  }
-};
-struct CtaCount {
-  int n;
-  template <typename Pred>
-  __device__ __forceinline__ int operator()(Pred pred) const {
-    int c = 0;
-    for (int i0 = 0; i0 < n; i0 += kThreads) {
-      const int i = i0 + static_cast<int>(threadIdx.x);
-      c += __syncthreads_count(i < n && pred(i));
-    }
-    return c;
-  }
-};
 
 struct Entry {
   uint32_t key, id;
@@ -288,15 +280,15 @@ template <typename T>
 __global__ void __launch_bounds__(kThreads, 5)
 k_token_logprobs(const __grid_constant__ Params p) {
   constexpr int kN = Vec<T>::kN;
-  extern __shared__ uint32_t s_keys[];             // segment maxima, as keys
+  extern __shared__ __align__(16) uint32_t s_keys[];      // segment maxima, as keys
   __shared__ Sums s_sums[kWarps];
   __shared__ Sums s_part;                          // this CTA's sums, read by rank 0
   __shared__ Entry s_best[kMaxTop];                // this CTA's best, in order; read by rank 0
   __shared__ int s_nbest;
-  __shared__ uint32_t s_run[kMaxTop];              // chosen segments, then chosen vectors
-  __shared__ uint32_t s_vec_key[kMaxTop * 32];
+  __shared__ uint32_t s_run[kMaxTop], s_vec[kMaxTop];     // chosen segments, chosen vectors of theirs
+  __shared__ __align__(16) uint32_t s_vec_key[kMaxTop * 32];
   __shared__ Entry s_cand[kMaxCands];
-  __shared__ Cut s_cut;
+  __shared__ uint32_t s_least;
   __shared__ int s_count;
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -405,6 +397,7 @@ k_token_logprobs(const __grid_constant__ Params p) {
     s_count = 0;
     s_nbest = 0;
   }
+  if (p.top > 0 && tid < 3) s_keys[seg1 - seg0 + tid] = 0u;
   __syncthreads();
   if (tid == 0) {
     Sums a = s_sums[0];
@@ -420,44 +413,44 @@ k_token_logprobs(const __grid_constant__ Params p) {
     const int n = seg1 - seg0;
     const int runs = min(want, n);
     constexpr int kBits = 32 - Key<T>::kLow;
-    auto itself = [](int i) { return i; };
     if (warp == 0) {
-      const Cut cut = find_cut<kBits>(s_keys, n, runs, WarpCount{n}, itself);
-      int at = 0;
-      for (int i0 = 0; i0 < n; i0 += 32) {
-        const int i = i0 + lane;
-        const uint32_t in = __ballot_sync(0xffffffffu, i < n && cut.chosen(s_keys[i < n ? i : 0], i));
-        if (in & (1u << lane)) s_run[at + __popc(in & ((1u << lane) - 1u))] = seg0 + i;
-        at += __popc(in);
-      }
-      if (lane == 0) s_cut = cut;
+      const uint32_t least = warp_select<kBits>(s_keys, n, runs, s_run);
+      if (lane == 0) s_least = least;
     }
     __syncthreads();
+    // A warp's candidates, appended together.
+    auto append = [&](bool in, uint32_t key, int id) {
+      const uint32_t ins = __ballot_sync(0xffffffffu, in);
+      if (ins == 0u) return;
+      int at = 0;
+      if (lane == 0) at = atomicAdd(&s_count, __popc(ins));
+      at = __shfl_sync(0xffffffffu, at, 0) + __popc(ins & ((1u << lane) - 1u));
+      if (in && at < kMaxCands) s_cand[at] = Entry{key, static_cast<uint32_t>(id)};
+    };
     // No value below the least of the chosen maxima is among the best: there are `runs` that are not.
-    // (Where all segments are chosen there is no such bound.)
-    const uint32_t least = n > want ? s_cut.key : 0u;
-    for (int j = warp; j < runs; j += kWarps) {
-      const int v = static_cast<int>(s_run[j]) * 32 + lane;
-      if (v < nvec) {
+    // (Where all segments are chosen there is no such bound, and the least is 0.)
+    const uint32_t least = n > want ? s_least : 0u;
+    if (n > want || (last - first) <= kMaxCands) {
+      for (int j = warp; j < runs; j += kWarps) {
+        const int v = (seg0 + static_cast<int>(s_run[j])) * 32 + lane;
         float f[kN];
-        Vec<T>::unpack(r.load(v), f);
+        Vec<T>::unpack(v < nvec ? r.load(v) : make_uint4(0u, 0u, 0u, 0u), f);
 #pragma unroll
         for (int e = 0; e < kN; ++e) {
           const int id = v * kN - r.head + e;
           const uint32_t key = order_key<T>(f[e]);
-          if (key >= least && id >= 0 && id < r.V) {
-            const int at = atomicAdd(&s_count, 1);
-            if (at < kMaxCands) s_cand[at] = Entry{key, static_cast<uint32_t>(id)};
-          }
+          append(key >= least && id >= 0 && id < r.V, key, id);
         }
       }
+    } else if (tid == 0) {
+      s_count = kMaxCands + 1;
     }
     __syncthreads();
     if (s_count > kMaxCands) {
       // Too many: the best vectors of these segments, each by its best value (0 where it holds none of the row).
       const int nv = runs * 32;
       for (int i = tid; i < nv; i += kThreads) {
-        const int v = static_cast<int>(s_run[i >> 5]) * 32 + (i & 31);
+        const int v = (seg0 + static_cast<int>(s_run[i >> 5])) * 32 + (i & 31);
         uint32_t key = 0;
         if (v < nvec) {
           float f[kN];
@@ -471,27 +464,17 @@ k_token_logprobs(const __grid_constant__ Params p) {
         s_vec_key[i] = key;
       }
       __syncthreads();
-      if (tid == 0) s_count = 0;
       const int vecs = min(want, nv);
-      auto vec_id = [&](int i) { return static_cast<int>(s_run[i >> 5]) * 32 + (i & 31); };
-      const Cut cut = find_cut<kBits>(s_vec_key, nv, vecs, CtaCount{nv}, vec_id);
-      uint32_t mine[kMaxTop * 32 / kThreads];
-#pragma unroll
-      for (int j = 0; j < kMaxTop * 32 / kThreads; ++j) {
-        const int i = tid + j * kThreads;
-        mine[j] = i < nv && cut.chosen(s_vec_key[i], vec_id(i)) ? vec_id(i) : 0xffffffffu;
+      if (warp == 0) {
+        warp_select<kBits>(s_vec_key, nv, vecs, s_vec);
+        if (lane == 0) s_count = 0;
       }
-      __syncthreads();                                 // s_run is read no more
-#pragma unroll
-      for (int j = 0; j < kMaxTop * 32 / kThreads; ++j)
-        if (mine[j] != 0xffffffffu) s_run[atomicAdd(&s_count, 1)] = mine[j];
       __syncthreads();
-      if (tid == 0) s_count = 0;
-      __syncthreads();
-      if (tid < vecs * kN) {
-        const int id = static_cast<int>(s_run[tid / kN]) * kN - r.head + tid % kN;
-        if (id >= 0 && id < r.V) s_cand[atomicAdd(&s_count, 1)] = Entry{order_key<T>(to_float(r.x[id])), static_cast<uint32_t>(id)};
-      }
+      const int at = tid / kN;
+      const int i = at < vecs ? static_cast<int>(s_vec[at]) : 0;
+      const int id = ((seg0 + static_cast<int>(s_run[i >> 5])) * 32 + (i & 31)) * kN - r.head + tid % kN;
+      const bool in = at < vecs && id >= 0 && id < r.V;
+      append(in, order_key<T>(in ? to_float(r.x[id]) : 0.f), id);
       __syncthreads();
     }
     const int cands = s_count;
@@ -570,7 +553,7 @@ int run(const Params& p, int64_t M, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(M * p.cluster));
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = p.top > 0 ? static_cast<size_t>(segments / p.cluster + 1) * 4 : 0;
+  cfg.dynamicSmemBytes = p.top > 0 ? static_cast<size_t>(segments / p.cluster + 4) * 4 : 0;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
