@@ -174,6 +174,19 @@ __device__ __forceinline__ Sums join(Sums a, Sums b) {
 }
 
 // ---------------------------------------------------------------- one row
+// The first n <= 8 of `parts` joined as a tree, the same one every time; all lanes of a warp.
+__device__ __forceinline__ Sums join_warps(const Sums* parts, int n) {
+  const int lane = threadIdx.x & 7;      // every eight lanes the same
+  Sums a = lane < n ? parts[lane] : Sums{-CUDART_INF_F, 0.f, 0.f};
+#pragma unroll
+  for (int o = 1; o < 8; o *= 2) {
+    const Sums b{__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.s, o),
+                 __shfl_xor_sync(0xffffffffu, a.t, o)};
+    a = (lane & o) ? join(b, a) : join(a, b);
+  }
+  return a;
+}
+
 template <typename T>
 struct Row {
   static constexpr int kN = Vec<T>::kN;
@@ -215,39 +228,104 @@ struct Row {
   }
 };
 
-// The indexes of the k best of keys[0, n), n >= k, equal ones by rising index, written to `out` in
-// rising order; one warp.  keys is 16-byte aligned, padded with zeros to a multiple of four.  Returns
-// the least of the chosen keys (0 when all are).  The threshold is searched bit by bit from the top and most
-// often found, as the first one that exactly k keys reach, long before the last bit.
+// A value and its id as one number: larger is better, and the lower id among equal values.
+__device__ __forceinline__ uint64_t entry(uint32_t key, uint32_t id) {
+  return (static_cast<uint64_t>(key) << 32) | (0xffffffffu - id);
+}
+__device__ __forceinline__ uint32_t entry_id(uint64_t e) { return 0xffffffffu - static_cast<uint32_t>(e); }
+__device__ __forceinline__ uint32_t entry_key(uint64_t e) { return static_cast<uint32_t>(e >> 32); }
+// How many of list[0, n) come before e; the list is padded with zeros to a multiple of eight.
+__device__ __forceinline__ int place_of(const uint64_t* list, int n, uint64_t e) {
+  int place = 0;
+  for (int i = 0; i < n; i += 8) {
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+      const ulonglong2 q = *reinterpret_cast<const ulonglong2*>(list + i + j);
+      place += (q.x > e) + (q.y > e);
+    }
+  }
+  return place;
+}
+
+constexpr int kPick = 128;      // what warp_select ranks by counting
+
+// The indexes of the k best of keys[0, n), n >= k, k <= 32, equal ones by rising index, written to
+// `out` in rising order; one warp.  keys is 16-byte aligned and padded with zeros to a multiple of four.
+// Returns the least of the chosen keys (0 when all are).
+//
+// The k-th best of the lanes' own maxima is a bound that k keys reach, and few more do: on values in
+// no order about 31 for k = 20, 112 for k = 32.  Those are ranked by counting.  Where more than 128 reach it
+// (ties), the threshold is searched bit by bit instead, 4 to 10 times as long.
 template <int kBits>
-__device__ uint32_t warp_select(const uint32_t* keys, int n, int k, uint32_t* out) {
+__device__ uint32_t warp_select(const uint32_t* keys, int n, int k, uint32_t* out, uint64_t* pick) {
   const int lane = threadIdx.x & 31;
-  auto count = [&](uint32_t least) {
+  const uint32_t below = (1u << lane) - 1u;
+  if (n <= k) {
+    if (lane < n) out[lane] = lane;
+    return 0u;
+  }
+  uint32_t mine = 0;
+#pragma unroll 8
+  for (int i = lane; i < n; i += 32) mine = max(mine, keys[i]);
+  int place = 0;
+#pragma unroll
+  for (int j = 0; j < 32; ++j) {
+    const uint32_t other = __shfl_sync(0xffffffffu, mine, j);
+    place += other > mine || (other == mine && j < lane);
+  }
+  uint32_t cut = __shfl_sync(0xffffffffu, mine, __ffs(__ballot_sync(0xffffffffu, place == k - 1)) - 1);
+  int found = 0;
+#pragma unroll 4
+  for (int i0 = 0; i0 < n; i0 += 32) {
+    const int i = i0 + lane;
+    const uint32_t key = i < n ? keys[i] : 0u;
+    const bool in = i < n && key >= cut;
+    const uint32_t ins = __ballot_sync(0xffffffffu, in);
+    const int at = found + __popc(ins & below);
+    if (in && at < kPick) pick[at] = entry(key, i);
+    found += __popc(ins);
+  }
+  if (found <= kPick) {
+    for (int i = found + lane; i < ((found + 7) & ~7); i += 32) pick[i] = 0;
+    __syncwarp();
+    uint32_t least = 0xffffffffu;
+    int at = 0;
+    for (int i0 = 0; i0 < found; i0 += 32) {
+      const uint64_t e = i0 + lane < found ? pick[i0 + lane] : 0;
+      const bool in = e != 0 && place_of(pick, found, e) < k;
+      const uint32_t ins = __ballot_sync(0xffffffffu, in);
+      if (in) {
+        out[at + __popc(ins & below)] = entry_id(e);
+        least = min(least, entry_key(e));
+      }
+      at += __popc(ins);
+    }
+    __syncwarp();
+    return __reduce_min_sync(0xffffffffu, least);
+  }
+  auto count = [&](uint32_t bound) {
     int c = 0;
 #pragma unroll 5
     for (int i = lane; i < (n + 3) / 4; i += 32) {
       const uint4 q = reinterpret_cast<const uint4*>(keys)[i];
-      c += (q.x >= least) + (q.y >= least) + (q.z >= least) + (q.w >= least);
+      c += (q.x >= bound) + (q.y >= bound) + (q.z >= bound) + (q.w >= bound);
     }
     return __reduce_add_sync(0xffffffffu, c);
   };
-  uint32_t cut = 0;
   int ties = n;                        // how many keys equal to the cut are taken
-  if (n > k) {
-    bool exact = false;
-    for (int b = kBits - 1; b >= 0 && !exact; --b) {
-      const uint32_t cand = cut | (1u << b);
-      const int c = count(cand);
-      if (c >= k) cut = cand;
-      exact = c == k;
-    }
-    if (!exact) ties = k - count(cut + 1u);
+  bool exact = false;
+  cut = 0;
+  for (int b = kBits - 1; b >= 0 && !exact; --b) {
+    const uint32_t cand = cut | (1u << b);
+    const int c = count(cand);
+    if (c >= k) cut = cand;
+    exact = c == k;
   }
+  if (!exact) ties = k - count(cut + 1u);
   int at = 0;
   for (int i0 = 0; i0 < n; i0 += 32) {
     const int i = i0 + lane;
     const uint32_t key = i < n ? keys[i] : 0u;
-    const uint32_t below = (1u << lane) - 1u;
     const uint32_t equal = __ballot_sync(0xffffffffu, i < n && key == cut);
     const bool in = i < n && (key > cut || (key == cut && __popc(equal & below) < ties));
     const uint32_t ins = __ballot_sync(0xffffffffu, in);
@@ -255,14 +333,8 @@ __device__ uint32_t warp_select(const uint32_t* keys, int n, int k, uint32_t* ou
     at += __popc(ins);
     ties = max(0, ties - __popc(equal));
   }
+  __syncwarp();
   return cut;
-}
-
-struct Entry {
-  uint32_t key, id;
-};
-__device__ __forceinline__ bool before(const Entry& a, const Entry& b) {
-  return a.key > b.key || (a.key == b.key && a.id < b.id);
 }
 
 struct Params {
@@ -283,11 +355,11 @@ k_token_logprobs(const __grid_constant__ Params p) {
   extern __shared__ __align__(16) uint32_t s_keys[];      // segment maxima, as keys
   __shared__ Sums s_sums[kWarps];
   __shared__ Sums s_part;                          // this CTA's sums, read by rank 0
-  __shared__ Entry s_best[kMaxTop];                // this CTA's best, in order; read by rank 0
-  __shared__ int s_nbest;
+  __shared__ __align__(16) uint64_t s_best[kMaxTop];      // this CTA's best, in order, then zeros; read by rank 0
   __shared__ uint32_t s_run[kMaxTop], s_vec[kMaxTop];     // chosen segments, chosen vectors of theirs
   __shared__ __align__(16) uint32_t s_vec_key[kMaxTop * 32];
-  __shared__ Entry s_cand[kMaxCands];
+  __shared__ __align__(16) uint64_t s_cand[kMaxCands];
+  __shared__ __align__(16) uint64_t s_pick[kPick];
   __shared__ uint32_t s_least;
   __shared__ int s_count;
 
@@ -393,16 +465,13 @@ k_token_logprobs(const __grid_constant__ Params p) {
     }
     if (lane == 0) s_sums[warp] = Sums{m, s, t};
   }
-  if (tid == 0) {
-    s_count = 0;
-    s_nbest = 0;
-  }
+  if (tid == 0) s_count = 0;
+  if (tid < kMaxTop) s_best[tid] = 0;
   if (p.top > 0 && tid < 3) s_keys[seg1 - seg0 + tid] = 0u;
   __syncthreads();
-  if (tid == 0) {
-    Sums a = s_sums[0];
-    for (int w = 1; w < kWarps; ++w) a = join(a, s_sums[w]);
-    s_part = a;
+  if (warp == kWarps - 1) {
+    const Sums a = join_warps(s_sums, kWarps);
+    if (lane == 0) s_part = a;
   }
 
   // -------------------------------------------------------------- alternatives
@@ -414,18 +483,29 @@ k_token_logprobs(const __grid_constant__ Params p) {
     const int runs = min(want, n);
     constexpr int kBits = 32 - Key<T>::kLow;
     if (warp == 0) {
-      const uint32_t least = warp_select<kBits>(s_keys, n, runs, s_run);
+      const uint32_t least = warp_select<kBits>(s_keys, n, runs, s_run, s_pick);
       if (lane == 0) s_least = least;
     }
     __syncthreads();
-    // A warp's candidates, appended together.
-    auto append = [&](bool in, uint32_t key, int id) {
-      const uint32_t ins = __ballot_sync(0xffffffffu, in);
-      if (ins == 0u) return;
+    // A warp's candidates, bit e of `in` for value e of a lane's vector, appended together.
+    auto append = [&](uint32_t in, const auto& key_of, int id0) {
+      if (__ballot_sync(0xffffffffu, in != 0) == 0u) return;
+      int sum = __popc(in);
+#pragma unroll
+      for (int o = 1; o < 32; o *= 2) {
+        const int up = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += up;
+      }
       int at = 0;
-      if (lane == 0) at = atomicAdd(&s_count, __popc(ins));
-      at = __shfl_sync(0xffffffffu, at, 0) + __popc(ins & ((1u << lane) - 1u));
-      if (in && at < kMaxCands) s_cand[at] = Entry{key, static_cast<uint32_t>(id)};
+      if (lane == 31) at = atomicAdd(&s_count, sum);
+      at = __shfl_sync(0xffffffffu, at, 31) + sum - __popc(in);
+#pragma unroll
+      for (int e = 0; e < kN; ++e) {
+        if (in & (1u << e)) {
+          if (at < kMaxCands) s_cand[at] = entry(key_of(e), static_cast<uint32_t>(id0 + e));
+          ++at;
+        }
+      }
     };
     // No value below the least of the chosen maxima is among the best: there are `runs` that are not.
     // (Where all segments are chosen there is no such bound, and the least is 0.)
@@ -435,12 +515,13 @@ k_token_logprobs(const __grid_constant__ Params p) {
         const int v = (seg0 + static_cast<int>(s_run[j])) * 32 + lane;
         float f[kN];
         Vec<T>::unpack(v < nvec ? r.load(v) : make_uint4(0u, 0u, 0u, 0u), f);
+        uint32_t in = 0;
 #pragma unroll
         for (int e = 0; e < kN; ++e) {
           const int id = v * kN - r.head + e;
-          const uint32_t key = order_key<T>(f[e]);
-          append(key >= least && id >= 0 && id < r.V, key, id);
+          if (order_key<T>(f[e]) >= least && id >= 0 && id < r.V) in |= 1u << e;
         }
+        append(in, [&](int e) { return order_key<T>(f[e]); }, v * kN - r.head);
       }
     } else if (tid == 0) {
       s_count = kMaxCands + 1;
@@ -466,7 +547,7 @@ k_token_logprobs(const __grid_constant__ Params p) {
       __syncthreads();
       const int vecs = min(want, nv);
       if (warp == 0) {
-        warp_select<kBits>(s_vec_key, nv, vecs, s_vec);
+        warp_select<kBits>(s_vec_key, nv, vecs, s_vec, s_pick);
         if (lane == 0) s_count = 0;
       }
       __syncthreads();
@@ -474,57 +555,66 @@ k_token_logprobs(const __grid_constant__ Params p) {
       const int i = at < vecs ? static_cast<int>(s_vec[at]) : 0;
       const int id = ((seg0 + static_cast<int>(s_run[i >> 5])) * 32 + (i & 31)) * kN - r.head + tid % kN;
       const bool in = at < vecs && id >= 0 && id < r.V;
-      append(in, order_key<T>(in ? to_float(r.x[id]) : 0.f), id);
+      append(in, [&](int) { return order_key<T>(to_float(r.x[id])); }, id);
       __syncthreads();
     }
     const int cands = s_count;
+    if (tid >= cands && tid < ((cands + 7) & ~7)) s_cand[tid] = 0;
+    __syncthreads();
     if (tid < cands) {
-      const Entry e = s_cand[tid];
-      int place = 0;
-      for (int i = 0; i < cands; ++i) place += before(s_cand[i], e);
+      const uint64_t e = s_cand[tid];
+      const int place = place_of(s_cand, cands, e);
       if (place < want) s_best[place] = e;
     }
-    if (tid == 0) s_nbest = want;
   }
   __syncthreads();
 
   // ---------------------------------------------------------------- the row
   Sums a = s_part;
-  int nbest = s_nbest;
-  const Entry* best = s_best;
   if (p.cluster > 1) {
     cluster_arrive();
     cluster_wait();
     if (rank == 0) {
-      // a warp for each CTA's part: its sums and its best, all at once; then ranked among all of them
+      // A warp to each CTA's part: its sums and its best, all at once.
       auto remote = [&](const void* local) {
         uint32_t v;
         asm volatile("ld.shared::cluster.u32 %0, [%1];"
                      : "=r"(v) : "r"(mapa_shared(smem_u32(local), static_cast<uint32_t>(warp))) : "memory");
         return v;
       };
+      uint64_t e = 0;
       if (warp < p.cluster) {
-        if (lane == 0)
-          s_sums[warp] = Sums{__uint_as_float(remote(&s_part.m)), __uint_as_float(remote(&s_part.s)),
-                              __uint_as_float(remote(&s_part.t))};
-        if (p.top > 0) {
-          const int nb = static_cast<int>(remote(&s_nbest));
-          // (this CTA's own list is read from its place too: s_cand is another array)
-          s_cand[tid] = lane < nb ? Entry{remote(&s_best[lane].key), remote(&s_best[lane].id)} : Entry{0u, 0xffffffffu};
+        if (lane < 3) reinterpret_cast<uint32_t*>(&s_sums[warp])[lane] = remote(reinterpret_cast<uint32_t*>(&s_part) + lane);
+        if (lane < p.top) {
+          const uint32_t* b = reinterpret_cast<const uint32_t*>(s_best + lane);
+          e = (static_cast<uint64_t>(remote(b + 1)) << 32) | remote(b);
         }
+        // each part's last bounds the row's last from below
+        if (lane == p.top - 1) s_pick[warp] = e;
       }
+      if (tid == 0) s_count = 0;
       __syncthreads();
-      a = s_sums[0];
-      for (int c = 1; c < p.cluster; ++c) a = join(a, s_sums[c]);      // in rank order
-      const int total = p.top > 0 ? p.cluster * kMaxTop : 0;
-      if (tid < total && s_cand[tid].key != 0u) {
-        const Entry e = s_cand[tid];
-        int place = 0;
-        for (int i = 0; i < total; ++i) place += before(s_cand[i], e);
-        if (place < p.top) s_best[place] = e;
+      a = join_warps(s_sums, p.cluster);
+      if (p.top > 0) {
+        uint64_t bound = 1;
+        for (int c = 0; c < p.cluster; ++c) bound = max(bound, static_cast<uint64_t>(s_pick[c]));
+        const bool in = e >= bound;
+        const uint32_t ins = __ballot_sync(0xffffffffu, in);
+        int at = 0;
+        if (lane == 0 && ins != 0u) at = atomicAdd(&s_count, __popc(ins));
+        at = __shfl_sync(0xffffffffu, at, 0) + __popc(ins & ((1u << lane) - 1u));
+        if (in) s_cand[at] = e;
+        __syncthreads();
+        const int total = s_count;
+        if (tid >= total && tid < ((total + 7) & ~7)) s_cand[tid] = 0;
+        __syncthreads();
+        if (tid < total) {
+          const uint64_t mine = s_cand[tid];
+          const int place = place_of(s_cand, total, mine);
+          if (place < p.top) s_best[place] = mine;
+        }
+        __syncthreads();
       }
-      nbest = p.top;
-      __syncthreads();
     }
   }
   if (rank == 0) {
@@ -534,10 +624,10 @@ k_token_logprobs(const __grid_constant__ Params p) {
       p.logprob[row] = (xt - a.m) - lse;
       p.entropy[row] = lse - a.t / a.s * kLn2;
     }
-    if (tid < nbest) {
-      const Entry e = best[tid];
-      p.top_ids[row * p.top + tid] = e.id;
-      p.top_logprobs[row * p.top + tid] = (key_value<T>(e.key) - a.m) - lse;
+    if (tid < p.top) {
+      const uint64_t e = s_best[tid];
+      p.top_ids[row * p.top + tid] = entry_id(e);
+      p.top_logprobs[row * p.top + tid] = (key_value<T>(entry_key(e)) - a.m) - lse;
     }
   }
   if (p.cluster > 1) {       // nobody leaves while its part is being read
