@@ -234,87 +234,44 @@ __device__ __forceinline__ uint64_t entry(uint32_t key, uint32_t id) {
 }
 __device__ __forceinline__ uint32_t entry_id(uint64_t e) { return 0xffffffffu - static_cast<uint32_t>(e); }
 __device__ __forceinline__ uint32_t entry_key(uint64_t e) { return static_cast<uint32_t>(e >> 32); }
-// How many of list[0, n) come before e; the list is padded with zeros to a multiple of eight.
-__device__ __forceinline__ int place_of(const uint64_t* list, int n, uint64_t e) {
+// How many of list[from, n) step by step of 2 * stride come before e; the list is padded with zeros to a
+// multiple of 4 * stride.
+template <int kStride>
+__device__ __forceinline__ int place_of(const uint64_t* list, int n, int from, uint64_t e) {
   int place = 0;
-  for (int i = 0; i < n; i += 8) {
+  for (int i = from; i < n; i += 4 * kStride) {
 #pragma unroll
-    for (int j = 0; j < 8; j += 2) {
-      const ulonglong2 q = *reinterpret_cast<const ulonglong2*>(list + i + j);
+    for (int j = 0; j < 2; ++j) {
+      const ulonglong2 q = *reinterpret_cast<const ulonglong2*>(list + i + 2 * j * kStride);
       place += (q.x > e) + (q.y > e);
     }
   }
   return place;
 }
 
-constexpr int kPick = 128;      // what warp_select ranks by counting
+constexpr int kPick = 128;      // what select ranks by counting, two threads to an entry
 
-// The indexes of the k best of keys[0, n), n >= k, k <= 32, equal ones by rising index, written to
-// `out` in rising order; one warp.  keys is 16-byte aligned and padded with zeros to a multiple of four.
-// Returns the least of the chosen keys (0 when all are).
-//
-// The k-th best of the lanes' own maxima is a bound that k keys reach, and few more do: on values in
-// no order about 31 for k = 20, 112 for k = 32.  Those are ranked by counting.  Where more than 128 reach it
-// (ties), the threshold is searched bit by bit instead, 4 to 10 times as long.
+struct SelectScratch {
+  uint64_t pick[kPick];
+  uint32_t tau[kWarps];
+  uint32_t least;
+  int found;
+};
+
+// The same by one warp, whatever the keys: the threshold is searched bit by bit from the top.
 template <int kBits>
-__device__ uint32_t warp_select(const uint32_t* keys, int n, int k, uint32_t* out, uint64_t* pick) {
+__device__ void search(const uint32_t* keys, int n, int k, uint32_t* out, SelectScratch& sc) {
   const int lane = threadIdx.x & 31;
   const uint32_t below = (1u << lane) - 1u;
-  if (n <= k) {
-    if (lane < n) out[lane] = lane;
-    return 0u;
-  }
-  uint32_t mine = 0;
-#pragma unroll 8
-  for (int i = lane; i < n; i += 32) mine = max(mine, keys[i]);
-  int place = 0;
-#pragma unroll
-  for (int j = 0; j < 32; ++j) {
-    const uint32_t other = __shfl_sync(0xffffffffu, mine, j);
-    place += other > mine || (other == mine && j < lane);
-  }
-  uint32_t cut = __shfl_sync(0xffffffffu, mine, __ffs(__ballot_sync(0xffffffffu, place == k - 1)) - 1);
-  int found = 0;
-#pragma unroll 4
-  for (int i0 = 0; i0 < n; i0 += 32) {
-    const int i = i0 + lane;
-    const uint32_t key = i < n ? keys[i] : 0u;
-    const bool in = i < n && key >= cut;
-    const uint32_t ins = __ballot_sync(0xffffffffu, in);
-    const int at = found + __popc(ins & below);
-    if (in && at < kPick) pick[at] = entry(key, i);
-    found += __popc(ins);
-  }
-  if (found <= kPick) {
-    for (int i = found + lane; i < ((found + 7) & ~7); i += 32) pick[i] = 0;
-    __syncwarp();
-    uint32_t least = 0xffffffffu;
-    int at = 0;
-    for (int i0 = 0; i0 < found; i0 += 32) {
-      const uint64_t e = i0 + lane < found ? pick[i0 + lane] : 0;
-      const bool in = e != 0 && place_of(pick, found, e) < k;
-      const uint32_t ins = __ballot_sync(0xffffffffu, in);
-      if (in) {
-        out[at + __popc(ins & below)] = entry_id(e);
-        least = min(least, entry_key(e));
-      }
-      at += __popc(ins);
-    }
-    __syncwarp();
-    return __reduce_min_sync(0xffffffffu, least);
-  }
   auto count = [&](uint32_t bound) {
     int c = 0;
-#pragma unroll 5
-    for (int i = lane; i < (n + 3) / 4; i += 32) {
-      const uint4 q = reinterpret_cast<const uint4*>(keys)[i];
-      c += (q.x >= bound) + (q.y >= bound) + (q.z >= bound) + (q.w >= bound);
-    }
+#pragma unroll 4
+    for (int i = lane; i < n; i += 32) c += keys[i] >= bound;
     return __reduce_add_sync(0xffffffffu, c);
   };
+  uint32_t cut = 0;
   int ties = n;                        // how many keys equal to the cut are taken
   bool exact = false;
-  cut = 0;
   for (int b = kBits - 1; b >= 0 && !exact; --b) {
     const uint32_t cand = cut | (1u << b);
     const int c = count(cand);
@@ -333,8 +290,60 @@ __device__ uint32_t warp_select(const uint32_t* keys, int n, int k, uint32_t* ou
     at += __popc(ins);
     ties = max(0, ties - __popc(equal));
   }
-  __syncwarp();
-  return cut;
+  if (lane == 0) sc.least = cut;
+}
+
+// The indexes of the k best of keys[0, n), equal ones by rising index, into out; k < n, k <= 32; the whole
+// CTA.  Leaves the least of the chosen keys in sc.least.
+//
+// Every warp holds an eighth of the keys and gives the ceil(k / 8)-th best of its lanes' own maxima; the
+// least of those is a bound that k keys reach, and few more do: some 50 for k = 20 on values in no
+// order.  They are ranked by counting.  Where more than 128 reach it (ties), one warp searches.
+template <int kBits>
+__device__ void select(const uint32_t* keys, int n, int k, uint32_t* out, SelectScratch& sc) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (tid == 0) sc.found = 0;
+  uint32_t mine = 0;
+  for (int i = lane * kWarps + warp; i < n; i += kThreads) mine = max(mine, keys[i]);
+  for (int j = kWarps; ; j += kWarps) {
+    const uint32_t top = __reduce_max_sync(0xffffffffu, mine);
+    if (j >= k) {
+      if (lane == 0) sc.tau[warp] = top;
+      break;
+    }
+    if (lane == __ffs(__ballot_sync(0xffffffffu, mine == top)) - 1) mine = 0;
+  }
+  __syncthreads();
+  uint32_t bound = sc.tau[lane & (kWarps - 1)];
+  bound = __reduce_min_sync(0xffffffffu, bound);
+  for (int i0 = 0; i0 < n; i0 += kThreads) {
+    const int i = i0 + lane * kWarps + warp;
+    const uint32_t key = i < n ? keys[i] : 0u;
+    const bool in = i < n && key >= bound;
+    const uint32_t ins = __ballot_sync(0xffffffffu, in);
+    if (ins != 0u) {
+      int at = 0;
+      if (lane == 0) at = atomicAdd(&sc.found, __popc(ins));
+      at = __shfl_sync(0xffffffffu, at, 0) + __popc(ins & ((1u << lane) - 1u));
+      if (in && at < kPick) sc.pick[at] = entry(key, i);
+    }
+  }
+  __syncthreads();
+  const int found = sc.found;
+  if (found <= kPick) {
+    if (tid >= found && tid < ((found + 7) & ~7)) sc.pick[tid] = 0;
+    __syncthreads();
+    const uint64_t e = tid / 2 < found ? sc.pick[tid / 2] : 0;
+    int place = place_of<2>(sc.pick, found, 2 * (tid & 1), e);
+    place += __shfl_xor_sync(0xffffffffu, place, 1);
+    if (e != 0 && place < k && (tid & 1) == 0) {
+      out[place] = entry_id(e);
+      if (place == k - 1) sc.least = entry_key(e);
+    }
+  } else if (warp == 0) {
+    search<kBits>(keys, n, k, out, sc);
+  }
+  __syncthreads();
 }
 
 struct Params {
@@ -359,8 +368,7 @@ k_token_logprobs(const __grid_constant__ Params p) {
   __shared__ uint32_t s_run[kMaxTop], s_vec[kMaxTop];     // chosen segments, chosen vectors of theirs
   __shared__ __align__(16) uint32_t s_vec_key[kMaxTop * 32];
   __shared__ __align__(16) uint64_t s_cand[kMaxCands];
-  __shared__ __align__(16) uint64_t s_pick[kPick];
-  __shared__ uint32_t s_least;
+  __shared__ __align__(16) SelectScratch s_select;
   __shared__ int s_count;
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -389,10 +397,11 @@ k_token_logprobs(const __grid_constant__ Params p) {
     float mx[kUnroll];
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) mx[u] = u < count ? warp_max(Vec<T>::max(q[u])) : -CUDART_INF_F;
-    if (p.top > 0 && lane == 0) {
+    if (p.top > 0 && lane < count) {          // a lane to a segment
+      float v = mx[0];
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u)
-        if (u < count) s_keys[seg + u * kWarps - seg0] = order_key<T>(mx[u]);
+      for (int u = 1; u < kUnroll; ++u) v = lane == u ? mx[u] : v;
+      s_keys[seg + lane * kWarps - seg0] = order_key<T>(v);
     }
     float grown = m;
 #pragma unroll
@@ -467,7 +476,6 @@ k_token_logprobs(const __grid_constant__ Params p) {
   }
   if (tid == 0) s_count = 0;
   if (tid < kMaxTop) s_best[tid] = 0;
-  if (p.top > 0 && tid < 3) s_keys[seg1 - seg0 + tid] = 0u;
   __syncthreads();
   if (warp == kWarps - 1) {
     const Sums a = join_warps(s_sums, kWarps);
@@ -482,11 +490,12 @@ k_token_logprobs(const __grid_constant__ Params p) {
     const int n = seg1 - seg0;
     const int runs = min(want, n);
     constexpr int kBits = 32 - Key<T>::kLow;
-    if (warp == 0) {
-      const uint32_t least = warp_select<kBits>(s_keys, n, runs, s_run, s_pick);
-      if (lane == 0) s_least = least;
+    if (n > want) {
+      select<kBits>(s_keys, n, want, s_run, s_select);
+    } else {
+      if (tid < n) s_run[tid] = tid;
+      __syncthreads();
     }
-    __syncthreads();
     // A warp's candidates, bit e of `in` for value e of a lane's vector, appended together.
     auto append = [&](uint32_t in, const auto& key_of, int id0) {
       if (__ballot_sync(0xffffffffu, in != 0) == 0u) return;
@@ -507,55 +516,75 @@ k_token_logprobs(const __grid_constant__ Params p) {
         }
       }
     };
-    // No value below the least of the chosen maxima is among the best: there are `runs` that are not.
-    // (Where all segments are chosen there is no such bound, and the least is 0.)
-    const uint32_t least = n > want ? s_least : 0u;
-    if (n > want || (last - first) <= kMaxCands) {
-      for (int j = warp; j < runs; j += kWarps) {
-        const int v = (seg0 + static_cast<int>(s_run[j])) * 32 + lane;
+    // No value below the least of the chosen maxima is among the best: there are `want` that are not.
+    // (Where all segments are chosen there is no such bound.)
+    const uint32_t least = n > want ? s_select.least : 0u;
+    auto id_of = [&](int run, int e) { return ((seg0 + static_cast<int>(s_run[run >> 5])) * 32 + (run & 31)) * kN - r.head + e; };
+    if (n > want || last - first <= kMaxCands) {
+      uint4 q[kMaxTop / kWarps];
+#pragma unroll
+      for (int u = 0; u < kMaxTop / kWarps; ++u) {
+        const int j = warp + u * kWarps;
+        const int v = j < runs ? (seg0 + static_cast<int>(s_run[j])) * 32 + lane : nvec;
+        q[u] = v < nvec ? r.load(v) : make_uint4(0u, 0u, 0u, 0u);
+      }
+#pragma unroll
+      for (int u = 0; u < kMaxTop / kWarps; ++u) {
+        const int j = warp + u * kWarps;
+        if (j >= runs) break;
+        const int id0 = id_of(j * 32 + lane, 0);
         float f[kN];
-        Vec<T>::unpack(v < nvec ? r.load(v) : make_uint4(0u, 0u, 0u, 0u), f);
+        Vec<T>::unpack(q[u], f);
         uint32_t in = 0;
 #pragma unroll
-        for (int e = 0; e < kN; ++e) {
-          const int id = v * kN - r.head + e;
-          if (order_key<T>(f[e]) >= least && id >= 0 && id < r.V) in |= 1u << e;
-        }
-        append(in, [&](int e) { return order_key<T>(f[e]); }, v * kN - r.head);
+        for (int e = 0; e < kN; ++e)
+          if (order_key<T>(f[e]) >= least && id0 + e >= 0 && id0 + e < r.V) in |= 1u << e;
+        append(in, [&](int e) { return order_key<T>(f[e]); }, id0);
       }
     } else if (tid == 0) {
       s_count = kMaxCands + 1;
     }
     __syncthreads();
     if (s_count > kMaxCands) {
-      // Too many: the best vectors of these segments, each by its best value (0 where it holds none of the row).
+      // Too many: the best vectors of these segments, each by its best value (0 where it holds none of the
+      // row), the segments in rising order so that a lower index is a lower id.
+      uint32_t run = 0;
+      int place = 0;
+      if (tid < runs) {
+        run = s_run[tid];
+        for (int j = 0; j < runs; ++j) place += s_run[j] < run;
+      }
+      __syncthreads();
+      if (tid < runs) s_run[place] = run;
+      __syncthreads();
       const int nv = runs * 32;
       for (int i = tid; i < nv; i += kThreads) {
-        const int v = (seg0 + static_cast<int>(s_run[i >> 5])) * 32 + (i & 31);
+        const int id0 = id_of(i, 0);
+        const int v = (id0 + r.head) / kN;
         uint32_t key = 0;
         if (v < nvec) {
           float f[kN];
           Vec<T>::unpack(r.load(v), f);
 #pragma unroll
-          for (int e = 0; e < kN; ++e) {
-            const int id = v * kN - r.head + e;
-            if (id >= 0 && id < r.V) key = max(key, order_key<T>(f[e]));
-          }
+          for (int e = 0; e < kN; ++e)
+            if (id0 + e >= 0 && id0 + e < r.V) key = max(key, order_key<T>(f[e]));
         }
         s_vec_key[i] = key;
       }
+      if (tid == 0) s_count = 0;
       __syncthreads();
       const int vecs = min(want, nv);
-      if (warp == 0) {
-        warp_select<kBits>(s_vec_key, nv, vecs, s_vec, s_pick);
-        if (lane == 0) s_count = 0;
+      if (nv > want) {
+        select<kBits>(s_vec_key, nv, want, s_vec, s_select);
+      } else {
+        if (tid < nv) s_vec[tid] = tid;
+        __syncthreads();
       }
-      __syncthreads();
+      const uint32_t least_of_vecs = nv > want ? s_select.least : 0u;
       const int at = tid / kN;
-      const int i = at < vecs ? static_cast<int>(s_vec[at]) : 0;
-      const int id = ((seg0 + static_cast<int>(s_run[i >> 5])) * 32 + (i & 31)) * kN - r.head + tid % kN;
-      const bool in = at < vecs && id >= 0 && id < r.V;
-      append(in, [&](int) { return order_key<T>(to_float(r.x[id])); }, id);
+      const int id = at < vecs ? id_of(static_cast<int>(s_vec[at]), tid % kN) : -1;
+      const uint32_t key = id >= 0 && id < r.V ? order_key<T>(to_float(r.x[id])) : 0u;
+      append(key != 0u && key >= least_of_vecs ? 1u : 0u, [&](int) { return key; }, id);
       __syncthreads();
     }
     const int cands = s_count;
@@ -563,7 +592,7 @@ k_token_logprobs(const __grid_constant__ Params p) {
     __syncthreads();
     if (tid < cands) {
       const uint64_t e = s_cand[tid];
-      const int place = place_of(s_cand, cands, e);
+      const int place = place_of<2>(s_cand, cands, 0, e) + place_of<2>(s_cand, cands, 2, e);
       if (place < want) s_best[place] = e;
     }
   }
@@ -590,14 +619,14 @@ k_token_logprobs(const __grid_constant__ Params p) {
           e = (static_cast<uint64_t>(remote(b + 1)) << 32) | remote(b);
         }
         // each part's last bounds the row's last from below
-        if (lane == p.top - 1) s_pick[warp] = e;
+        if (lane == p.top - 1) s_select.pick[warp] = e;
       }
       if (tid == 0) s_count = 0;
       __syncthreads();
       a = join_warps(s_sums, p.cluster);
       if (p.top > 0) {
         uint64_t bound = 1;
-        for (int c = 0; c < p.cluster; ++c) bound = max(bound, static_cast<uint64_t>(s_pick[c]));
+        for (int c = 0; c < p.cluster; ++c) bound = max(bound, s_select.pick[c]);
         const bool in = e >= bound;
         const uint32_t ins = __ballot_sync(0xffffffffu, in);
         int at = 0;
@@ -610,7 +639,7 @@ k_token_logprobs(const __grid_constant__ Params p) {
         __syncthreads();
         if (tid < total) {
           const uint64_t mine = s_cand[tid];
-          const int place = place_of(s_cand, total, mine);
+          const int place = place_of<2>(s_cand, total, 0, mine) + place_of<2>(s_cand, total, 2, mine);
           if (place < p.top) s_best[place] = mine;
         }
         __syncthreads();
@@ -643,7 +672,7 @@ int run(const Params& p, int64_t M, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(M * p.cluster));
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = p.top > 0 ? static_cast<size_t>(segments / p.cluster + 4) * 4 : 0;
+  cfg.dynamicSmemBytes = p.top > 0 ? static_cast<size_t>(segments / p.cluster + 1) * 4 : 0;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
