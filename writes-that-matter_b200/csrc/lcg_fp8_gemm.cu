@@ -11,6 +11,7 @@
 //                   the column side, K is split over a cluster, bound by reading the weight once.
 #include <cuda_bf16.h>
 
+#include <atomic>
 #include <cstring>
 
 #include "lcg_common.h"
@@ -381,20 +382,23 @@ k_gemm_fp8(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CU
 }
 
 // ================================================================= few rows
-// 6 warps: 0 TMA producer, 1 MMA issuer, 2-5 read-back.  A CTA multiplies 128 rows of the weight by
-// kBT tokens over its share of the K blocks; the CTAs of a cluster share one tile's K and add their
-// parts in rank order through distributed shared memory.
+// Warps: 0 TMA producer, 1 MMA issuer, 2-5 (2-9 for 128 tokens) read-back, 64 tokens at most to a warp.  A
+// CTA multiplies 128 rows of the weight by kBT tokens over its share of the K blocks; the CTAs of a
+// cluster share one tile's K and add their parts in rank order through distributed shared memory.
 template <int kBT>
 struct Few {
   static constexpr int kStageBytes = kOperandBytes + kBT * kBlock;
-  static constexpr int kStages = kBT == 16 ? 6 : kBT == 32 ? 5 : kBT == 64 ? 4 : 3;   // two CTAs to an SM
-  static constexpr int kAcc = kBT == 128 ? 2 : 4;
+  static constexpr int kCtas = kBT == 128 ? 1 : 2;          // CTAs to an SM
+  static constexpr int kStages = kBT == 16 ? 6 : kBT == 32 ? 5 : kBT == 64 ? 4 : 6;
+  static constexpr int kReaders = kBT == 128 ? 8 : 4;       // read-back warps
+  static constexpr int kThreads = 64 + 32 * kReaders;
+  static constexpr int kCols = kBT * 4 / kReaders;          // tokens to a warp
+  static constexpr int kAcc = 4;
   static constexpr int kTmemCols = kAcc * kBT;
   static constexpr int kAhead = 4;                          // K blocks whose scales are staged together
   static constexpr int kScaleBytes = 2 * kAhead * kBT * 4;
   static constexpr int kSmemBytes = kStages * kStageBytes + kScaleBytes + 256 + 1024;
 };
-constexpr int kFewThreads = 192;
 constexpr int kMaxSplit = 8;
 
 struct FewParams {
@@ -406,7 +410,7 @@ struct FewParams {
 };
 
 template <int kBT>
-__global__ void __launch_bounds__(kFewThreads, 2)
+__global__ void __launch_bounds__(Few<kBT>::kThreads, Few<kBT>::kCtas)
 k_gemm_fp8_few(const __grid_constant__ CUtensorMap tma_w, const __grid_constant__ CUtensorMap tma_x,
                const __grid_constant__ FewParams p) {
   using T = Few<kBT>;
@@ -444,7 +448,7 @@ k_gemm_fp8_few(const __grid_constant__ CUtensorMap tma_w, const __grid_constant_
     }
     for (uint32_t s = 0; s < T::kAcc; ++s) {
       mbar_init(acc_full_bar(s), 1);
-      mbar_init(acc_empty_bar(s), 4);
+      mbar_init(acc_empty_bar(s), T::kReaders);
     }
     misc_gen[1] = 0u;
     fence_mbar_init();
@@ -505,85 +509,102 @@ k_gemm_fp8_few(const __grid_constant__ CUtensorMap tma_w, const __grid_constant_
     }
   } else {
     // ---------------------------------------------------------------- read-back
+    constexpr int kReadThreads = 32 * T::kReaders;
     const int quarter = warp & 3;
     const int row = quarter * 32 + lane;
+    const int tok0 = ((warp - 2) >> 2) * T::kCols;         // this warp's first token of the tile
     const int pt = threadIdx.x - 64;
-    const uint32_t lane_addr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
-    // Scales of kAhead blocks at a time, a's times b's, staged by all four warps: [block][token].
-    constexpr int kPer = (T::kAhead * kBT + 127) / 128;
+    const uint32_t lane_addr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + tok0;
+    // Scales of kAhead blocks at a time, a's times b's, staged by all the read-back warps: [block][token].
+    constexpr int kPer = (T::kAhead * kBT + kReadThreads - 1) / kReadThreads;
     float na[kPer], nb[kPer];
     const float* sb = p.b.p + tn * p.b.row;
     auto fetch = [&](int kbs) {
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
-        const int e = pt + i * 128;
+        const int e = pt + i * kReadThreads;
         const int kb = kbs + e / kBT, j = e % kBT;
         const bool in = e < T::kAhead * kBT && kb < kb1 && j < tokens;
         na[i] = in ? __ldg(p.a.p + (m0 + j) * p.a.row + kb * p.a.blk) : 0.f;
         nb[i] = in ? __ldg(sb + kb * p.b.blk) : 0.f;
       }
     };
-    uint64_t acc[kBT / 2];
+    uint64_t acc[T::kCols / 2];
 #pragma unroll
-    for (int j = 0; j < kBT / 2; ++j) acc[j] = 0;
+    for (int j = 0; j < T::kCols / 2; ++j) acc[j] = 0;
     uint32_t as = 0, acc_parity = 0;
     fetch(kb0);
+    constexpr int kChunks = T::kCols / 16;
+    uint32_t v[2][16];
+    mbar_wait_inline(acc_full_bar(as), acc_parity, ctl, kCodeEpilogue);
+    tcgen05_fence_after();
+    tmem_ld_32x16(lane_addr, v[0]);
     int flip = 0;
     for (int kbs = kb0; kbs < kb1; kbs += T::kAhead, flip ^= 1) {
       float* stage_s = scales + flip * T::kAhead * kBT;
 #pragma unroll
       for (int i = 0; i < kPer; ++i)
-        if (pt + i * 128 < T::kAhead * kBT) stage_s[pt + i * 128] = na[i] * nb[i];
+        if (pt + i * kReadThreads < T::kAhead * kBT) stage_s[pt + i * kReadThreads] = na[i] * nb[i];
       // past this barrier every warp is done with the other half, which the next round overwrites
-      bar_sync(1, 128);
+      bar_sync(1, kReadThreads);
       fetch(kbs + T::kAhead);
-#pragma unroll 1
-      for (int i = 0; i < T::kAhead && kbs + i < kb1; ++i) {
-        mbar_wait_inline(acc_full_bar(as), acc_parity, ctl, kCodeEpilogue);
-        tcgen05_fence_after();
-        const ulonglong2* s4 = reinterpret_cast<const ulonglong2*>(stage_s + i * kBT);
 #pragma unroll
-        for (int c = 0; c < kBT / 16; ++c) {
-          uint32_t v[16];
-          tmem_ld_32x16(lane_addr + as * kBT + c * 16, v);
-          tmem_ld_wait(v);
-          if (c + 1 == kBT / 16) {
-            tcgen05_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(acc_empty_bar(as));
-          }
+      for (int i = 0; i < T::kAhead; ++i) {
+        if (kbs + i < kb1) {
+          const ulonglong2* s4 = reinterpret_cast<const ulonglong2*>(stage_s + i * kBT + tok0);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const ulonglong2 s = s4[c * 4 + j];
-            acc[c * 8 + 2 * j] = fma_f32x2(pack_f32x2(v[4 * j], v[4 * j + 1]), s.x, acc[c * 8 + 2 * j]);
-            acc[c * 8 + 2 * j + 1] = fma_f32x2(pack_f32x2(v[4 * j + 2], v[4 * j + 3]), s.y, acc[c * 8 + 2 * j + 1]);
+          for (int c = 0; c < kChunks; ++c) {
+            // one load in flight ahead of its use, across the stages too (as in k_gemm_fp8)
+            uint32_t (&u)[16] = v[(i * kChunks + c) & 1];
+            uint32_t (&w)[16] = v[(i * kChunks + c + 1) & 1];
+            ulonglong2 sc[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) sc[j] = s4[c * 4 + j];
+            tmem_ld_wait(u);
+            if (c + 1 < kChunks) {
+              tmem_ld_32x16(lane_addr + as * kBT + (c + 1) * 16, w);
+            } else {
+              tcgen05_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(acc_empty_bar(as));
+              if (++as == T::kAcc) {
+                as = 0;
+                acc_parity ^= 1u;
+              }
+              if (kbs + i + 1 < kb1) {
+                mbar_wait_inline(acc_full_bar(as), acc_parity, ctl, kCodeEpilogue);
+                tcgen05_fence_after();
+                tmem_ld_32x16(lane_addr + as * kBT, w);
+              }
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              acc[c * 8 + 2 * j] = fma_f32x2(pack_f32x2(u[4 * j], u[4 * j + 1]), sc[j].x, acc[c * 8 + 2 * j]);
+              acc[c * 8 + 2 * j + 1] = fma_f32x2(pack_f32x2(u[4 * j + 2], u[4 * j + 3]), sc[j].y, acc[c * 8 + 2 * j + 1]);
+            }
           }
-        }
-        if (++as == T::kAcc) {
-          as = 0;
-          acc_parity ^= 1u;
         }
       }
     }
     if (p.split == 1) {
       if (n0 + row < p.n) {
 #pragma unroll
-        for (int j = 0; j < kBT / 2; ++j) {
+        for (int j = 0; j < T::kCols / 2; ++j) {
           float lo, hi;
           unpack_f32x2(acc[j], lo, hi);
-          __nv_bfloat16* dst = p.c + static_cast<int64_t>(m0 + 2 * j) * p.ldc + n0 + row;
-          if (2 * j < tokens) dst[0] = __float2bfloat16_rn(lo);
-          if (2 * j + 1 < tokens) dst[p.ldc] = __float2bfloat16_rn(hi);
+          __nv_bfloat16* dst = p.c + static_cast<int64_t>(m0 + tok0 + 2 * j) * p.ldc + n0 + row;
+          if (tok0 + 2 * j < tokens) dst[0] = __float2bfloat16_rn(lo);
+          if (tok0 + 2 * j + 1 < tokens) dst[p.ldc] = __float2bfloat16_rn(hi);
         }
       }
     } else {
       // The last product is complete, so the operand stages are free to hold the partial sums.
 #pragma unroll
-      for (int j = 0; j < kBT / 2; ++j) {
+      for (int j = 0; j < T::kCols / 2; ++j) {
         float lo, hi;
         unpack_f32x2(acc[j], lo, hi);
-        part[(2 * j) * kTileRows + row] = lo;
-        part[(2 * j + 1) * kTileRows + row] = hi;
+        part[(tok0 + 2 * j) * kTileRows + row] = lo;
+        part[(tok0 + 2 * j + 1) * kTileRows + row] = hi;
       }
     }
   }
@@ -593,9 +614,12 @@ k_gemm_fp8_few(const __grid_constant__ CUtensorMap tma_w, const __grid_constant_
   if (p.split > 1) {
     cluster_arrive();
     cluster_wait();
-    const int row = threadIdx.x;
-    if (row < kTileRows && n0 + row < p.n) {
-      for (int j = rank; j < tokens; j += p.split) {
+    // rank r joins the tokens r, r + split, ..., a half of the CTA to every other one of them
+    const int row = threadIdx.x & (kTileRows - 1);
+    const int half = threadIdx.x >> 7;
+    constexpr int kHalves = T::kThreads / kTileRows;
+    if (half < kHalves && n0 + row < p.n) {
+      for (int j = rank + half * p.split; j < tokens; j += kHalves * p.split) {
         const uint32_t addr = base + static_cast<uint32_t>(j * kTileRows + row) * 4u;
         float sum = 0.f;
         for (int r = 0; r < p.split; ++r) {
@@ -713,12 +737,35 @@ int run_few(const Call& q) {
   p.token_tiles = static_cast<int32_t>((q.m + kBT - 1) / kBT);
   p.status = q.status;
   const int64_t tiles = static_cast<int64_t>(p.token_tiles) * ((q.n + kTileRows - 1) / kTileRows);
-  // Split K so that the slots (two CTAs to an SM) are filled: rounds of CTAs times the K blocks of each.
-  const int slots = 2 * sm_count();
+  // Split K so that the GPU is filled: rounds of clusters times the K blocks of a CTA.  How many clusters of
+  // a size run at once is asked once per device: the GPU's parts are not multiples of each size
+  // (40 clusters of 7 need two rounds on 148 SMs with two CTAs each: 25 us, where 40 of 6 take 20.6).
+  static bool configured[64] = {};
+  if (int e = configure(k_gemm_fp8_few<kBT>, T::kSmemBytes, configured)) return e;
+  static std::atomic<int> at_once[64][kMaxSplit + 1];
+  int dev = 0;
+  LCG_CUDA_OK(cudaGetDevice(&dev));
   int split = 1;
   double best = 1e30;
   for (int s = 1; s <= kMaxSplit && s <= p.k_blocks; ++s) {
-    const double rounds = static_cast<double>((tiles * s + slots - 1) / slots);
+    int clusters = dev >= 0 && dev < 64 ? at_once[dev][s].load(std::memory_order_relaxed) : 0;
+    if (clusters == 0) {
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3(static_cast<unsigned>(s));
+      cfg.blockDim = dim3(T::kThreads);
+      cfg.dynamicSmemBytes = T::kSmemBytes;
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = static_cast<unsigned>(s);
+      attr[0].val.clusterDim.y = 1;
+      attr[0].val.clusterDim.z = 1;
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      LCG_CUDA_OK(cudaOccupancyMaxActiveClusters(&clusters, k_gemm_fp8_few<kBT>, &cfg));
+      if (clusters < 1) clusters = 1;
+      if (dev >= 0 && dev < 64) at_once[dev][s].store(clusters, std::memory_order_relaxed);
+    }
+    const double rounds = static_cast<double>((tiles + clusters - 1) / clusters);
     const double cost = rounds * ((p.k_blocks + s - 1) / s) + 0.5 * s;      // a rank to add costs half a block's time
     if (cost < best) {
       best = cost;
@@ -727,9 +774,7 @@ int run_few(const Call& q) {
   }
   p.split = split;
   if (tiles * split > 0x7fffffffLL) return fail(LCG_ERR_UNSUPPORTED_SHAPE, "too many tiles");
-  static bool configured[64] = {};
-  if (int e = configure(k_gemm_fp8_few<kBT>, T::kSmemBytes, configured)) return e;
-  return launch(k_gemm_fp8_few<kBT>, static_cast<unsigned>(tiles * split), kFewThreads, T::kSmemBytes,
+  return launch(k_gemm_fp8_few<kBT>, static_cast<unsigned>(tiles * split), T::kThreads, T::kSmemBytes,
                 static_cast<unsigned>(split), q.stream, mw, mx, p);
 }
 
