@@ -738,8 +738,9 @@ int run_few(const Call& q) {
   p.status = q.status;
   const int64_t tiles = static_cast<int64_t>(p.token_tiles) * ((q.n + kTileRows - 1) / kTileRows);
   // Split K so that the GPU is filled: rounds of clusters times the K blocks of a CTA.  How many clusters of
-  // a size run at once is asked once per device: the GPU's parts are not multiples of each size
-  // (40 clusters of 7 need two rounds on 148 SMs with two CTAs each: 25 us, where 40 of 6 take 20.6).
+  // a size run at once is asked once per device, for one CTA to an SM as the runtime counts them: the
+  // GPU's parts are not multiples of each size (15 of 7, 22 of 6; 5120 x 17408 and one token, 40
+  // clusters: 25.1 us with 7 in two rounds, 20.8 with 6 in one).
   static bool configured[64] = {};
   if (int e = configure(k_gemm_fp8_few<kBT>, T::kSmemBytes, configured)) return e;
   static std::atomic<int> at_once[64][kMaxSplit + 1];
@@ -765,6 +766,7 @@ int run_few(const Call& q) {
       if (clusters < 1) clusters = 1;
       if (dev >= 0 && dev < 64) at_once[dev][s].store(clusters, std::memory_order_relaxed);
     }
+    clusters *= T::kCtas;
     const double rounds = static_cast<double>((tiles + clusters - 1) / clusters);
     const double cost = rounds * ((p.k_blocks + s - 1) / s) + 0.5 * s;      // a rank to add costs half a block's time
     if (cost < best) {
