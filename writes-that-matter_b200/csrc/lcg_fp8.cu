@@ -44,19 +44,38 @@ __device__ __forceinline__ uint32_t amax_bits8(const float (&f)[8]) {
   return m;
 }
 
-// Two fp32 values -> two e4m3 codes, `lo` in the low byte.
-__device__ __forceinline__ uint32_t cvt_e4m3x2(float lo, float hi) {
-  uint16_t r;
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+// Four fp32 values, scaled, -> four e4m3 codes, the first in the low byte.
+__device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d, uint64_t inv2) {
+  uint32_t r;
+  asm("{\n\t"
+      ".reg .b64 p, q;\n\t"
+      ".reg .b32 a, b, c, d;\n\t"
+      ".reg .b16 l, h;\n\t"
+      "mov.b64 p, {%1, %2};\n\t"
+      "mov.b64 q, {%3, %4};\n\t"
+      "mul.rn.f32x2 p, p, %5;\n\t"
+      "mul.rn.f32x2 q, q, %5;\n\t"
+      "mov.b64 {a, b}, p;\n\t"
+      "mov.b64 {c, d}, q;\n\t"
+      "cvt.rn.satfinite.e4m3x2.f32 l, b, a;\n\t"
+      "cvt.rn.satfinite.e4m3x2.f32 h, d, c;\n\t"
+      "mov.b32 %0, {l, h};\n\t"
+      "}"
+      : "=r"(r) : "f"(a), "f"(b), "f"(c), "f"(d), "l"(inv2));
   return r;
 }
 __device__ __forceinline__ uint2 encode8(const float (&f)[8], float inv) {
-  uint2 o;
-  o.x = cvt_e4m3x2(__fmul_rn(f[0], inv), __fmul_rn(f[1], inv)) |
-        (cvt_e4m3x2(__fmul_rn(f[2], inv), __fmul_rn(f[3], inv)) << 16);
-  o.y = cvt_e4m3x2(__fmul_rn(f[4], inv), __fmul_rn(f[5], inv)) |
-        (cvt_e4m3x2(__fmul_rn(f[6], inv), __fmul_rn(f[7], inv)) << 16);
-  return o;
+  uint64_t inv2;
+  asm("mov.b64 %0, {%1, %1};" : "=l"(inv2) : "f"(inv));
+  return make_uint2(encode4(f[0], f[1], f[2], f[3], inv2), encode4(f[4], f[5], f[6], f[7], inv2));
+}
+
+// 448 / a for the 16 lanes of a block, and in its odd lanes a / 448, the block's scale: one division, of
+// different operands in even and odd lanes, as both are as long as half the rest of a block's work.
+__device__ __forceinline__ float inverse_and_scale(float a, float& scale) {
+  const bool odd = threadIdx.x & 1;
+  scale = (odd ? a : kTop) / (odd ? kTop : a);
+  return __shfl_sync(0xffffffffu, scale, (threadIdx.x & 31) & ~1);
 }
 
 // Maximum over the 16 lanes that hold one block (eight values each).
@@ -66,16 +85,34 @@ __device__ __forceinline__ uint32_t block_max16(uint32_t bits) {
   return max(bits, kFloorBits);
 }
 
-__device__ __forceinline__ uint4 load8(const __nv_bfloat16* p, int64_t left, bool vec) {
+// Read once: past L1.
+__device__ __forceinline__ uint4 ldg_stream(const __nv_bfloat16* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+
+__device__ __forceinline__ uint4 load8(const __nv_bfloat16* p, int left, bool vec) {
   // `left`: values of the row from p on; what lies past them reads as zero.
   if (left <= 0) return make_uint4(0u, 0u, 0u, 0u);
-  if (vec && left >= 8) return __ldg(reinterpret_cast<const uint4*>(p));
+  if (vec && left >= 8) return ldg_stream(p);
   uint32_t w[4] = {0u, 0u, 0u, 0u};
   const unsigned short* s = reinterpret_cast<const unsigned short*>(p);
 #pragma unroll
   for (int e = 0; e < 8; ++e)
     if (e < left) w[e >> 1] |= static_cast<uint32_t>(s[e]) << (16 * (e & 1));
   return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// The (row, block) of the groups of 16 lanes that a CTA takes in turn, 16 apart.  All in 32 bits.
+struct Walk {
+  uint32_t groups, kblocks, step_row, step_blk;      // 16 = step_row * kblocks + step_blk
+};
+__device__ __forceinline__ void advance(const Walk& w, uint32_t& row, uint32_t& blk) {
+  row += w.step_row;
+  blk += w.step_blk;
+  if (blk >= w.kblocks) blk -= w.kblocks, ++row;
 }
 
 struct ScaleOut {
@@ -85,148 +122,205 @@ struct ScaleOut {
 
 // Codes of eight values at column `col` of a row: the row's pitch is a multiple of 16 bytes, and
 // the columns past K up to that multiple are written as zeros.
-__device__ __forceinline__ void store8(uint8_t* row, int64_t col, int64_t kpad, const uint2& o) {
+__device__ __forceinline__ void store8(uint8_t* row, int col, int kpad, const uint2& o) {
   if (col < kpad) *reinterpret_cast<uint2*>(row + col) = o;
 }
 
-// One 16-lane group per (row, block); 16 groups per CTA.
+// A 16-lane group to a block, 16 groups to a CTA, kRowUnroll blocks in turn to a group with all their
+// loads in flight (4096 x 5120: one block at a time 19 us).
+constexpr int kRowUnroll = 4;
 __global__ void __launch_bounds__(256)
-k_quantize_rows(const __nv_bfloat16* __restrict__ x, int64_t groups, int64_t K, int64_t ldx, uint32_t kblocks,
-                bool vec, uint8_t* __restrict__ q, int64_t ldq, ScaleOut sc) {
-  const int64_t g = static_cast<int64_t>(blockIdx.x) * 16 + (threadIdx.x >> 4);
+k_quantize_rows(const __nv_bfloat16* __restrict__ x, const Walk w, int K, int64_t ldx, bool vec,
+                uint8_t* __restrict__ q, int64_t ldq, ScaleOut sc) {
+  const uint32_t g0 = blockIdx.x * (16u * kRowUnroll) + (threadIdx.x >> 4);
   const int sub = threadIdx.x & 15;
-  const bool live = g < groups;
-  const int64_t gg = live ? g : 0;
-  const int64_t row = gg / kblocks;
-  const int64_t blk = gg - row * kblocks;
-  const int64_t col = blk * kBlock + sub * 8;
-  const uint4 v = load8(x + row * ldx + col, K - col, vec);
-  const float a = __uint_as_float(block_max16(amax_bits8(v)));
-  if (!live) return;
-  float f[8];
-  unpack8(v, f);
-  store8(q + row * ldq, col, (K + 15) & ~int64_t(15), encode8(f, kTop / a));
-  if (sub == 0) sc.p[row * sc.row + blk * sc.blk] = a / kTop;
+  const int kpad = (K + 15) & ~15;
+  const uint32_t row0 = g0 / w.kblocks, blk0 = g0 - row0 * w.kblocks;
+  uint4 v[kRowUnroll];
+  uint32_t row = row0, blk = blk0;
+#pragma unroll
+  for (int j = 0; j < kRowUnroll; ++j) {
+    const int col = static_cast<int>(blk) * kBlock + sub * 8;
+    v[j] = load8(x + row * ldx + col, g0 + 16 * j < w.groups ? K - col : 0, vec);
+    advance(w, row, blk);
+  }
+  row = row0;
+  blk = blk0;
+#pragma unroll
+  for (int j = 0; j < kRowUnroll; ++j) {
+    const float a = __uint_as_float(block_max16(amax_bits8(v[j])));
+    float scale;
+    const float inv = inverse_and_scale(a, scale);
+    if (g0 + 16 * j < w.groups) {
+      float f[8];
+      unpack8(v[j], f);
+      store8(q + row * ldq, static_cast<int>(blk) * kBlock + sub * 8, kpad, encode8(f, inv));
+      if (sub == 1) sc.p[row * sc.row + blk * sc.blk] = scale;
+    }
+    advance(w, row, blk);
+  }
 }
 
-// One CTA per 128 x 128 tile: 256 threads hold eight vectors of eight values each.
-__global__ void __launch_bounds__(256)
-k_quantize_tiles(const __nv_bfloat16* __restrict__ x, int64_t M, int64_t K, int64_t ldx, bool vec,
+// A CTA to two neighbouring 128 x 128 tiles, a warp to 512 contiguous bytes of a row (one tile to a CTA,
+// with 256 bytes of each row, took 78 us for 5120 x 17408): 512 threads hold eight vectors of eight values
+// each, lanes 0-15 of the left tile and 16-31 of the right one.
+__global__ void __launch_bounds__(512)
+k_quantize_tiles(const __nv_bfloat16* __restrict__ x, int64_t M, int K, int64_t ldx, bool vec,
                  uint8_t* __restrict__ q, int64_t ldq, ScaleOut sc) {
-  __shared__ uint32_t s_max[8];
-  const int64_t col = static_cast<int64_t>(blockIdx.x) * kBlock + (threadIdx.x & 15) * 8;
-  const int64_t row0 = static_cast<int64_t>(blockIdx.y) * kBlock + (threadIdx.x >> 4);
+  __shared__ uint32_t s_max[2][16];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, side = lane >> 4;
+  const int col = static_cast<int>(blockIdx.x) * (2 * kBlock) + lane * 8;
+  const int64_t row0 = static_cast<int64_t>(blockIdx.y) * kBlock + warp;
+  const int rows = static_cast<int>(min(static_cast<int64_t>(kBlock), M - static_cast<int64_t>(blockIdx.y) * kBlock)) - warp;
+  const __nv_bfloat16* p = x + row0 * ldx + col;
   uint4 v[8];
   uint32_t bits = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int64_t row = row0 + 16 * i;
-    v[i] = load8(x + row * ldx + col, row < M ? K - col : 0, vec);
-    bits = max(bits, amax_bits8(v[i]));
-  }
-  bits = __reduce_max_sync(0xffffffffu, bits);
-  if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = bits;
+  for (int i = 0; i < 8; ++i) v[i] = load8(p + 16 * i * ldx, 16 * i < rows ? K - col : 0, vec);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) bits = max(bits, amax_bits8(v[i]));
+  bits = block_max16(bits);
+  if ((lane & 15) == 0) s_max[side][warp] = bits;
   __syncthreads();
-  bits = kFloorBits;
-#pragma unroll
-  for (int w = 0; w < 8; ++w) bits = max(bits, s_max[w]);
-  const float a = __uint_as_float(bits);
-  const float inv = kTop / a;
+  bits = block_max16(s_max[side][lane & 15]);
+  float scale;
+  const float inv = inverse_and_scale(__uint_as_float(bits), scale);
+  uint8_t* o = q + row0 * ldq;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const int64_t row = row0 + 16 * i;
-    if (row >= M) continue;
-    float f[8];
-    unpack8(v[i], f);
-    store8(q + row * ldq, col, (K + 15) & ~int64_t(15), encode8(f, inv));
+    if (16 * i < rows) {
+      float f[8];
+      unpack8(v[i], f);
+      store8(o + 16 * i * ldq, col, (K + 15) & ~15, encode8(f, inv));
+    }
   }
-  if (threadIdx.x == 0) sc.p[blockIdx.y * sc.row + blockIdx.x * sc.blk] = a / kTop;
+  const int blk = 2 * static_cast<int>(blockIdx.x) + side;
+  if (warp == 0 && (lane & 15) == 1 && blk * kBlock < K) sc.p[blockIdx.y * sc.row + blk * sc.blk] = scale;
 }
 
 // h = bf16(delta + residual) -> residual_out, y = h * rsqrt(mean h^2 + eps) * (w + 1) quantised
-// from its fp32 value.  One CTA per row, kVpt vectors of eight values per thread held from the
-// load to the conversion; vector i of a thread is vector tid + i * blockDim of the row, and
-// blockDim is a multiple of 32, so the 16 lanes of a block stay together.
-template <int kVpt>
+// from its fp32 value.  kRows rows to a CTA, kVpt vectors of eight values of each to a thread, all loaded
+// before the first is used and held, packed, to the conversion; vector i of a thread is vector tid + i *
+// blockDim of the row, and blockDim is a multiple of 32, so the 16 lanes of a block stay together.
+template <int kRows, int kVpt>
 __global__ void __launch_bounds__(1024)
 k_add_rmsnorm_fp8(const __nv_bfloat16* __restrict__ delta, const __nv_bfloat16* residual,
-                  const __nv_bfloat16* __restrict__ w, int K, float eps, __nv_bfloat16* residual_out,
+                  const __nv_bfloat16* __restrict__ w, int64_t M, int K, float eps, __nv_bfloat16* residual_out,
                   uint8_t* __restrict__ q, int64_t ldq, ScaleOut sc) {
-  __shared__ float s_part[32];
-  const int64_t row = blockIdx.x;
+  __shared__ float s_part[kRows][32];
+  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * kRows;
   const int nvec = K / 8;
   const int tid = threadIdx.x, lane = tid & 31;
-  float h[kVpt][8];
-  float ss = 0.f;
+  uint4 h[kRows][kVpt], d[kRows][kVpt];
 #pragma unroll
-  for (int i = 0; i < kVpt; ++i) {
-    const int v = tid + i * static_cast<int>(blockDim.x);
-    uint4 r = make_uint4(0u, 0u, 0u, 0u);
-    if (v < nvec) {
-      r = *reinterpret_cast<const uint4*>(residual + row * K + v * 8);
+  for (int r = 0; r < kRows; ++r)
+#pragma unroll
+    for (int i = 0; i < kVpt; ++i) {
+      const int v = tid + i * static_cast<int>(blockDim.x);
+      const bool in = v < nvec && row0 + r < M;
+      const int64_t at = (row0 + r) * K + v * 8;
+      h[r][i] = in ? *reinterpret_cast<const uint4*>(residual + at) : make_uint4(0u, 0u, 0u, 0u);
+      if (delta != nullptr) d[r][i] = in ? ldg_stream(delta + at) : make_uint4(0u, 0u, 0u, 0u);
+    }
+#pragma unroll
+  for (int r = 0; r < kRows; ++r) {
+    float ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < kVpt; ++i) {
+      const int v = tid + i * static_cast<int>(blockDim.x);
+      float hf[8];
+      unpack8(h[r][i], hf);
       if (delta != nullptr) {
-        const uint4 d = __ldg(reinterpret_cast<const uint4*>(delta + row * K + v * 8));
-        float df[8], rf[8];
-        unpack8(d, df);
-        unpack8(r, rf);
+        float df[8];
+        unpack8(d[r][i], df);
         uint32_t o[4];
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-          const __nv_bfloat162 p = __floats2bfloat162_rn(df[2 * t] + rf[2 * t], df[2 * t + 1] + rf[2 * t + 1]);
+          const __nv_bfloat162 p = __floats2bfloat162_rn(df[2 * t] + hf[2 * t], df[2 * t + 1] + hf[2 * t + 1]);
           o[t] = *reinterpret_cast<const uint32_t*>(&p);
         }
-        r = make_uint4(o[0], o[1], o[2], o[3]);
-        *reinterpret_cast<uint4*>(residual_out + row * K + v * 8) = r;
+        h[r][i] = make_uint4(o[0], o[1], o[2], o[3]);
+        if (v < nvec && row0 + r < M) *reinterpret_cast<uint4*>(residual_out + (row0 + r) * K + v * 8) = h[r][i];
+        unpack8(h[r][i], hf);
       }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) ss = fmaf(hf[e], hf[e], ss);
     }
-    unpack8(r, h[i]);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) ss = fmaf(h[i][e], h[i][e], ss);
+    for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    if (lane == 0) s_part[r][tid >> 5] = ss;
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-  if (lane == 0) s_part[tid >> 5] = ss;
   __syncthreads();
-  float part = lane < static_cast<int>(blockDim.x >> 5) ? s_part[lane] : 0.f;
+  float rstd[kRows];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
-  const float rstd = rsqrtf(part / static_cast<float>(K) + eps);
+  for (int r = 0; r < kRows; ++r) {
+    float part = lane < static_cast<int>(blockDim.x >> 5) ? s_part[r][lane] : 0.f;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
+    rstd[r] = rsqrtf(part / static_cast<float>(K) + eps);
+  }
 #pragma unroll
   for (int i = 0; i < kVpt; ++i) {
     const int v = tid + i * static_cast<int>(blockDim.x);
     float wf[8];
     unpack8(v < nvec ? __ldg(reinterpret_cast<const uint4*>(w + v * 8)) : make_uint4(0u, 0u, 0u, 0u), wf);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) h[i][e] = h[i][e] * rstd * (wf[e] + 1.0f);
-    // past the row's end h is 0: such a value is 0, or NaN where rstd is, as its block then is
-    const float a = __uint_as_float(block_max16(v < nvec ? amax_bits8(h[i]) : 0u));
-    store8(q + row * ldq, v * 8, (K + 15) & ~15, v < nvec ? encode8(h[i], kTop / a) : make_uint2(0u, 0u));
-    if ((v & 15) == 0 && v < nvec) sc.p[row * sc.row + (v >> 4) * sc.blk] = a / kTop;
+    for (int r = 0; r < kRows; ++r) {
+      float y[8];
+      unpack8(h[r][i], y);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = y[e] * rstd[r] * (wf[e] + 1.0f);
+      // past the row's end h is 0: such a value is 0, or NaN where rstd is, as its block then is
+      const float a = __uint_as_float(block_max16(v < nvec ? amax_bits8(y) : 0u));
+      float scale;
+      const float inv = inverse_and_scale(a, scale);
+      if (row0 + r < M) {
+        store8(q + (row0 + r) * ldq, v * 8, (K + 15) & ~15, v < nvec ? encode8(y, inv) : make_uint2(0u, 0u));
+        if ((v & 15) == 1 && v - 1 < nvec) sc.p[(row0 + r) * sc.row + (v >> 4) * sc.blk] = scale;
+      }
+    }
   }
 }
 
-// silu(g) * u quantised from its fp32 value; silu(g) = g / (1 + e^-g).  One 16-lane group per
-// (row, block) of the result.
+// silu(g) * u quantised from its fp32 value; silu(g) = g / (1 + e^-g).  A 16-lane group to a block of the
+// result, kGluUnroll blocks in turn with all their loads in flight (4096 x 17408: one at a time 82 us).
+constexpr int kGluUnroll = 2;
 __global__ void __launch_bounds__(256)
-k_swiglu_fp8(const __nv_bfloat16* __restrict__ z, int64_t groups, int64_t inter, int64_t ldz, uint32_t kblocks,
+k_swiglu_fp8(const __nv_bfloat16* __restrict__ z, const Walk w, int inter, int64_t ldz,
              uint8_t* __restrict__ q, int64_t ldq, ScaleOut sc) {
-  const int64_t g = static_cast<int64_t>(blockIdx.x) * 16 + (threadIdx.x >> 4);
+  const uint32_t g0 = blockIdx.x * (16u * kGluUnroll) + (threadIdx.x >> 4);
   const int sub = threadIdx.x & 15;
-  const bool live = g < groups;
-  const int64_t gg = live ? g : 0;
-  const int64_t row = gg / kblocks;
-  const int64_t blk = gg - row * kblocks;
-  const int64_t col = blk * kBlock + sub * 8;
-  const __nv_bfloat16* p = z + row * ldz + col;
-  float gf[8], uf[8];
-  unpack8(load8(p, inter - col, true), gf);
-  unpack8(load8(p + inter, inter - col, true), uf);
+  const int ipad = (inter + 15) & ~15;
+  const uint32_t row0 = g0 / w.kblocks, blk0 = g0 - row0 * w.kblocks;
+  uint4 gv[kGluUnroll], uv[kGluUnroll];
+  uint32_t row = row0, blk = blk0;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) gf[e] = __fdividef(gf[e], 1.0f + __expf(-gf[e])) * uf[e];
-  const float a = __uint_as_float(block_max16(amax_bits8(gf)));
-  if (!live) return;
-  store8(q + row * ldq, col, (inter + 15) & ~int64_t(15), encode8(gf, kTop / a));
-  if (sub == 0) sc.p[row * sc.row + blk * sc.blk] = a / kTop;
+  for (int j = 0; j < kGluUnroll; ++j) {
+    const int col = static_cast<int>(blk) * kBlock + sub * 8;
+    const __nv_bfloat16* p = z + row * ldz + col;
+    const int left = g0 + 16 * j < w.groups ? inter - col : 0;
+    gv[j] = load8(p, left, true);
+    uv[j] = load8(p + inter, left, true);
+    advance(w, row, blk);
+  }
+  row = row0;
+  blk = blk0;
+#pragma unroll
+  for (int j = 0; j < kGluUnroll; ++j) {
+    float gf[8], uf[8];
+    unpack8(gv[j], gf);
+    unpack8(uv[j], uf);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) gf[e] = __fdividef(gf[e], 1.0f + __expf(-gf[e])) * uf[e];
+    const float a = __uint_as_float(block_max16(amax_bits8(gf)));
+    float scale;
+    const float inv = inverse_and_scale(a, scale);
+    if (g0 + 16 * j < w.groups) {
+      store8(q + row * ldq, static_cast<int>(blk) * kBlock + sub * 8, ipad, encode8(gf, inv));
+      if (sub == 1) sc.p[row * sc.row + blk * sc.blk] = scale;
+    }
+    advance(w, row, blk);
+  }
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -241,11 +335,14 @@ int check_codes(const void* q, int64_t ldq, int64_t K, const float* scale) {
   return LCG_OK;
 }
 
-int group_grid(int64_t M, int64_t kblocks, unsigned* grid) {
-  const int64_t ctas = (M * kblocks + 15) / 16;
-  if (M > (int64_t(1) << 40) / kblocks || ctas > 0x7fffffffLL)
+int make_walk(int64_t M, int64_t kblocks, int unroll, Walk* w, unsigned* grid) {
+  if (M > 0x40000000LL / kblocks)
     return fail(LCG_ERR_UNSUPPORTED_SHAPE, "too many blocks: M=%lld, %lld blocks a row", (long long)M, (long long)kblocks);
-  *grid = static_cast<unsigned>(ctas);
+  w->groups = static_cast<uint32_t>(M * kblocks);
+  w->kblocks = static_cast<uint32_t>(kblocks);
+  w->step_row = 16u / w->kblocks;
+  w->step_blk = 16u % w->kblocks;
+  *grid = (w->groups + 16 * unroll - 1) / (16 * unroll);
   return LCG_OK;
 }
 
@@ -271,14 +368,14 @@ extern "C" int lcg_quantize_fp8(const void* x, int64_t M, int64_t K, int64_t ldx
   auto xb = static_cast<const __nv_bfloat16*>(x);
   if (block_rows == 1) {
     unsigned grid;
-    if (int e = group_grid(M, kblocks, &grid)) return e;
-    k_quantize_rows<<<grid, 256, 0, st>>>(xb, M * kblocks, K, ldx, static_cast<uint32_t>(kblocks), vec,
-                                          static_cast<uint8_t*>(q), ldq, sc);
+    Walk w;
+    if (int e = make_walk(M, kblocks, kRowUnroll, &w, &grid)) return e;
+    k_quantize_rows<<<grid, 256, 0, st>>>(xb, w, static_cast<int>(K), ldx, vec, static_cast<uint8_t*>(q), ldq, sc);
   } else {
     const int64_t rblocks = (M + kBlock - 1) / kBlock;
     if (rblocks > 65535) return fail(LCG_ERR_UNSUPPORTED_SHAPE, "too many rows: M=%lld", (long long)M);
-    k_quantize_tiles<<<dim3(static_cast<unsigned>(kblocks), static_cast<unsigned>(rblocks)), 256, 0, st>>>(
-        xb, M, K, ldx, vec, static_cast<uint8_t*>(q), ldq, sc);
+    k_quantize_tiles<<<dim3(static_cast<unsigned>((kblocks + 1) / 2), static_cast<unsigned>(rblocks)), 512, 0, st>>>(
+        xb, M, static_cast<int>(K), ldx, vec, static_cast<uint8_t*>(q), ldq, sc);
   }
   LCG_CUDA_OK(cudaGetLastError());
   count_launch();
@@ -301,10 +398,15 @@ extern "C" int lcg_add_rmsnorm_fp8(const void* delta, const void* residual, cons
   // whole 16-byte groups of codes: the vectors are rounded up to an even count, the threads to whole warps
   const int threads = (((nvec + 1) / 2 * 2 + vpt - 1) / vpt + 31) / 32 * 32;
   const ScaleOut sc{scale, scale_row_stride, scale_block_stride};
-  auto kern = vpt == 1 ? k_add_rmsnorm_fp8<1> : vpt == 2 ? k_add_rmsnorm_fp8<2> : k_add_rmsnorm_fp8<3>;
-  kern<<<static_cast<unsigned>(M), threads, 0, static_cast<cudaStream_t>(stream)>>>(
+  // Two rows to a CTA once that still gives every SM two CTAs.
+  const bool two = vpt == 1 && M >= 4 * sm_count();
+  auto kern = two        ? k_add_rmsnorm_fp8<2, 1>
+              : vpt == 1 ? k_add_rmsnorm_fp8<1, 1>
+              : vpt == 2 ? k_add_rmsnorm_fp8<1, 2>
+                         : k_add_rmsnorm_fp8<1, 3>;
+  kern<<<static_cast<unsigned>(two ? (M + 1) / 2 : M), threads, 0, static_cast<cudaStream_t>(stream)>>>(
       static_cast<const __nv_bfloat16*>(delta), static_cast<const __nv_bfloat16*>(residual),
-      static_cast<const __nv_bfloat16*>(norm_weight), static_cast<int>(K), eps,
+      static_cast<const __nv_bfloat16*>(norm_weight), M, static_cast<int>(K), eps,
       static_cast<__nv_bfloat16*>(residual_out), static_cast<uint8_t*>(q), ldq, sc);
   LCG_CUDA_OK(cudaGetLastError());
   count_launch();
@@ -321,10 +423,11 @@ extern "C" int lcg_swiglu_fp8(const void* z, int64_t M, int64_t I, int64_t ldz, 
   if (int e = check_codes(q, ldq, I, scale)) return e;
   const int64_t kblocks = (I + kBlock - 1) / kBlock;
   unsigned grid;
-  if (int e = group_grid(M, kblocks, &grid)) return e;
+  Walk w;
+  if (int e = make_walk(M, kblocks, kGluUnroll, &w, &grid)) return e;
   k_swiglu_fp8<<<grid, 256, 0, static_cast<cudaStream_t>(stream)>>>(
-      static_cast<const __nv_bfloat16*>(z), M * kblocks, I, ldz, static_cast<uint32_t>(kblocks),
-      static_cast<uint8_t*>(q), ldq, ScaleOut{scale, scale_row_stride, scale_block_stride});
+      static_cast<const __nv_bfloat16*>(z), w, static_cast<int>(I), ldz, static_cast<uint8_t*>(q), ldq,
+      ScaleOut{scale, scale_row_stride, scale_block_stride});
   LCG_CUDA_OK(cudaGetLastError());
   count_launch();
   return LCG_OK;
