@@ -37,11 +37,14 @@ __device__ __forceinline__ uint32_t amax_bits8(const uint4& q) {
                               __vmaxu2(q.z & 0x7fff7fffu, q.w & 0x7fff7fffu));
   return max(m << 16, m & 0xffff0000u);
 }
+__device__ __forceinline__ float max3_abs(float a, float b, float c) {      // a NaN stays one
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(fabsf(a)), "f"(fabsf(b)), "f"(fabsf(c)));
+  return r;
+}
 __device__ __forceinline__ uint32_t amax_bits8(const float (&f)[8]) {
-  uint32_t m = 0;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) m = max(m, __float_as_uint(f[e]) & 0x7fffffffu);
-  return m;
+  const float m = max3_abs(max3_abs(f[0], f[1], f[2]), max3_abs(f[3], f[4], f[5]), max3_abs(f[6], f[7], f[7]));
+  return __float_as_uint(m) & 0x7fffffffu;
 }
 
 // Four fp32 values, scaled, -> four e4m3 codes, the first in the low byte.
@@ -199,86 +202,110 @@ k_quantize_tiles(const __nv_bfloat16* __restrict__ x, int64_t M, int K, int64_t 
 }
 
 // h = bf16(delta + residual) -> residual_out, y = h * rsqrt(mean h^2 + eps) * (w + 1) quantised
-// from its fp32 value.  kRows rows to a CTA, kVpt vectors of eight values of each to a thread, all loaded
-// before the first is used and held, packed, to the conversion; vector i of a thread is vector tid + i *
-// blockDim of the row, and blockDim is a multiple of 32, so the 16 lanes of a block stay together.
-template <int kRows, int kVpt>
-__global__ void __launch_bounds__(1024)
+// from its fp32 value.  One 16-lane group holds a block throughout, eight values to a lane.
+
+__device__ __forceinline__ uint4 add_bf16x8(const uint4& x, const uint4& y) {
+  float a[8], b[8];
+  unpack8(x, a);
+  unpack8(y, b);
+  uint32_t o[4];
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    const __nv_bfloat162 p = __floats2bfloat162_rn(a[2 * t] + b[2 * t], a[2 * t + 1] + b[2 * t + 1]);
+    o[t] = *reinterpret_cast<const uint32_t*>(&p);
+  }
+  return make_uint4(o[0], o[1], o[2], o[3]);
+}
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+// Squares of eight values added to two running sums.
+__device__ __forceinline__ void add_squares(const uint4& h, uint64_t& ss) {
+  float f[8];
+  unpack8(h, f);
+#pragma unroll
+  for (int e = 0; e < 8; e += 2) {
+    const uint64_t p = pair(f[e], f[e + 1]);
+    asm("fma.rn.f32x2 %0, %1, %1, %0;" : "+l"(ss) : "l"(p));
+  }
+}
+__device__ __forceinline__ float sum_warp(uint64_t ss) {
+  float lo, hi;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(ss));
+  lo += hi;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) lo += __shfl_xor_sync(0xffffffffu, lo, o);
+  return lo;
+}
+// Vector v of a normalised row: quantised and stored.  All lanes; `in`: the vector lies in the row.
+// Past the row's end h is 0: such a value is 0, or NaN where rstd is, as its block then is.
+__device__ __forceinline__ void norm_store(const uint4& h, const uint4& w, float rstd, int v, bool in, int kpad,
+                                           uint8_t* row, float* scales, int64_t blk_stride) {
+  float y[8], wf[8];
+  unpack8(h, y);
+  unpack8(w, wf);
+  const uint64_t one = pair(1.f, 1.f), r2 = pair(rstd, rstd);
+#pragma unroll
+  for (int e = 0; e < 8; e += 2) {
+    uint64_t a = pair(y[e], y[e + 1]), b = pair(wf[e], wf[e + 1]);
+    asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(a) : "l"(r2));
+    asm("add.rn.f32x2 %0, %0, %1;" : "+l"(b) : "l"(one));
+    asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(a) : "l"(b));
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(y[e]), "=f"(y[e + 1]) : "l"(a));
+  }
+  const float a = __uint_as_float(block_max16(in ? amax_bits8(y) : 0u));
+  float scale;
+  const float inv = inverse_and_scale(a, scale);
+  store8(row, v * 8, kpad, in ? encode8(y, inv) : make_uint2(0u, 0u));
+  if ((v & 15) == 1 && v * 8 - 8 < kpad) scales[(v >> 4) * blk_stride] = scale;
+}
+
+// A CTA of at most 512 threads to a row, kVpt vectors to a thread: vector i of a thread is vector
+// tid + i * blockDim of the row (blockDim a multiple of 32, so that a block's lanes stay together).  Two
+// vectors rather than one (8192 x 5120 with a delta: 54.6 us against 48.4) halve what the reduction over
+// the row costs, which every warp pays; a warp to a row pays it once but leaves 11 warps on an SM (127 us).
+constexpr int kNormThreads = 512;
+template <int kVpt>
+__global__ void __launch_bounds__(kNormThreads, kVpt == 2 ? 4 : kVpt == 4 ? 2 : 1)
 k_add_rmsnorm_fp8(const __nv_bfloat16* __restrict__ delta, const __nv_bfloat16* residual,
-                  const __nv_bfloat16* __restrict__ w, int64_t M, int K, float eps, __nv_bfloat16* residual_out,
+                  const __nv_bfloat16* __restrict__ w, int K, float inv_k, float eps, __nv_bfloat16* residual_out,
                   uint8_t* __restrict__ q, int64_t ldq, ScaleOut sc) {
-  __shared__ float s_part[kRows][32];
-  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * kRows;
+  __shared__ float s_part[32];
+  const int64_t row = blockIdx.x;
   const int nvec = K / 8;
   const int tid = threadIdx.x, lane = tid & 31;
-  uint4 h[kRows][kVpt], d[kRows][kVpt];
-#pragma unroll
-  for (int r = 0; r < kRows; ++r)
-#pragma unroll
-    for (int i = 0; i < kVpt; ++i) {
-      const int v = tid + i * static_cast<int>(blockDim.x);
-      const bool in = v < nvec && row0 + r < M;
-      const int64_t at = (row0 + r) * K + v * 8;
-      h[r][i] = in ? *reinterpret_cast<const uint4*>(residual + at) : make_uint4(0u, 0u, 0u, 0u);
-      if (delta != nullptr) d[r][i] = in ? ldg_stream(delta + at) : make_uint4(0u, 0u, 0u, 0u);
-    }
-#pragma unroll
-  for (int r = 0; r < kRows; ++r) {
-    float ss = 0.f;
-#pragma unroll
-    for (int i = 0; i < kVpt; ++i) {
-      const int v = tid + i * static_cast<int>(blockDim.x);
-      float hf[8];
-      unpack8(h[r][i], hf);
-      if (delta != nullptr) {
-        float df[8];
-        unpack8(d[r][i], df);
-        uint32_t o[4];
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          const __nv_bfloat162 p = __floats2bfloat162_rn(df[2 * t] + hf[2 * t], df[2 * t + 1] + hf[2 * t + 1]);
-          o[t] = *reinterpret_cast<const uint32_t*>(&p);
-        }
-        h[r][i] = make_uint4(o[0], o[1], o[2], o[3]);
-        if (v < nvec && row0 + r < M) *reinterpret_cast<uint4*>(residual_out + (row0 + r) * K + v * 8) = h[r][i];
-        unpack8(h[r][i], hf);
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) ss = fmaf(hf[e], hf[e], ss);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    if (lane == 0) s_part[r][tid >> 5] = ss;
-  }
-  __syncthreads();
-  float rstd[kRows];
-#pragma unroll
-  for (int r = 0; r < kRows; ++r) {
-    float part = lane < static_cast<int>(blockDim.x >> 5) ? s_part[r][lane] : 0.f;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
-    rstd[r] = rsqrtf(part / static_cast<float>(K) + eps);
-  }
+  const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+  uint4 h[kVpt], d[kVpt], wv[kVpt];
 #pragma unroll
   for (int i = 0; i < kVpt; ++i) {
     const int v = tid + i * static_cast<int>(blockDim.x);
-    float wf[8];
-    unpack8(v < nvec ? __ldg(reinterpret_cast<const uint4*>(w + v * 8)) : make_uint4(0u, 0u, 0u, 0u), wf);
+    h[i] = v < nvec ? *reinterpret_cast<const uint4*>(residual + row * K + v * 8) : zero;
+    if (delta != nullptr) d[i] = v < nvec ? ldg_stream(delta + row * K + v * 8) : zero;
+    wv[i] = v < nvec ? __ldg(reinterpret_cast<const uint4*>(w + v * 8)) : zero;
+  }
+  uint64_t ss = 0;
 #pragma unroll
-    for (int r = 0; r < kRows; ++r) {
-      float y[8];
-      unpack8(h[r][i], y);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] = y[e] * rstd[r] * (wf[e] + 1.0f);
-      // past the row's end h is 0: such a value is 0, or NaN where rstd is, as its block then is
-      const float a = __uint_as_float(block_max16(v < nvec ? amax_bits8(y) : 0u));
-      float scale;
-      const float inv = inverse_and_scale(a, scale);
-      if (row0 + r < M) {
-        store8(q + (row0 + r) * ldq, v * 8, (K + 15) & ~15, v < nvec ? encode8(y, inv) : make_uint2(0u, 0u));
-        if ((v & 15) == 1 && v - 1 < nvec) sc.p[(row0 + r) * sc.row + (v >> 4) * sc.blk] = scale;
-      }
+  for (int i = 0; i < kVpt; ++i) {
+    const int v = tid + i * static_cast<int>(blockDim.x);
+    if (delta != nullptr) {
+      h[i] = add_bf16x8(d[i], h[i]);
+      if (v < nvec) *reinterpret_cast<uint4*>(residual_out + row * K + v * 8) = h[i];
     }
+    add_squares(h[i], ss);
+  }
+  float part = sum_warp(ss);
+  if (lane == 0) s_part[tid >> 5] = part;
+  __syncthreads();
+  part = lane < static_cast<int>(blockDim.x >> 5) ? s_part[lane] : 0.f;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
+  const float rstd = rsqrtf(fmaf(part, inv_k, eps));
+#pragma unroll
+  for (int i = 0; i < kVpt; ++i) {
+    const int v = tid + i * static_cast<int>(blockDim.x);
+    norm_store(h[i], wv[i], rstd, v, v < nvec, (K + 15) & ~15, q + row * ldq, sc.p + row * sc.row, sc.blk);
   }
 }
 
@@ -394,20 +421,19 @@ extern "C" int lcg_add_rmsnorm_fp8(const void* delta, const void* residual, cons
     return fail(LCG_ERR_MISALIGNED, "all operands must be 16-byte aligned");
   if (int e = check_codes(q, ldq, K, scale)) return e;
   const int nvec = static_cast<int>(K / 8);
-  const int vpt = (nvec + 1023) / 1024;
-  // whole 16-byte groups of codes: the vectors are rounded up to an even count, the threads to whole warps
-  const int threads = (((nvec + 1) / 2 * 2 + vpt - 1) / vpt + 31) / 32 * 32;
   const ScaleOut sc{scale, scale_row_stride, scale_block_stride};
-  // Two rows to a CTA once that still gives every SM two CTAs.
-  const bool two = vpt == 1 && M >= 4 * sm_count();
-  auto kern = two        ? k_add_rmsnorm_fp8<2, 1>
-              : vpt == 1 ? k_add_rmsnorm_fp8<1, 1>
-              : vpt == 2 ? k_add_rmsnorm_fp8<1, 2>
-                         : k_add_rmsnorm_fp8<1, 3>;
-  kern<<<static_cast<unsigned>(two ? (M + 1) / 2 : M), threads, 0, static_cast<cudaStream_t>(stream)>>>(
-      static_cast<const __nv_bfloat16*>(delta), static_cast<const __nv_bfloat16*>(residual),
-      static_cast<const __nv_bfloat16*>(norm_weight), M, static_cast<int>(K), eps,
-      static_cast<__nv_bfloat16*>(residual_out), static_cast<uint8_t*>(q), ldq, sc);
+  auto st = static_cast<cudaStream_t>(stream);
+  auto db = static_cast<const __nv_bfloat16*>(delta), rb = static_cast<const __nv_bfloat16*>(residual),
+       wb = static_cast<const __nv_bfloat16*>(norm_weight);
+  auto ho = static_cast<__nv_bfloat16*>(residual_out);
+  auto qb = static_cast<uint8_t*>(q);
+  const float inv_k = 1.0f / static_cast<float>(K);
+  // vectors of the row and of the codes' padding to a multiple of 16
+  const int nslots = (nvec + 1) / 2 * 2;
+  const int vpt = nslots <= 2 * kNormThreads ? 2 : nslots <= 4 * kNormThreads ? 4 : 6;
+  const int threads = ((nslots + vpt - 1) / vpt + 31) / 32 * 32;
+  auto kern = vpt == 2 ? k_add_rmsnorm_fp8<2> : vpt == 4 ? k_add_rmsnorm_fp8<4> : k_add_rmsnorm_fp8<6>;
+  kern<<<static_cast<unsigned>(M), threads, 0, st>>>(db, rb, wb, static_cast<int>(K), inv_k, eps, ho, qb, ldq, sc);
   LCG_CUDA_OK(cudaGetLastError());
   count_launch();
   return LCG_OK;
