@@ -1307,7 +1307,7 @@ def run_model(args, device):
     rank-7 MLP, on seeded uniform-random prompts of 2048 / 4096 / 8192 tokens.  Times come from the
     first prompt of a length; agreement (equal top-1, tie-aware top-20 count, final hidden state)
     is taken over `--prompts` seeded prompts per length and reported as rates, for the rank-7 arm,
-    for its bit-reproducible all-ranks form, and for the calibration pair `eager` vs `stock` (two
+    for its bit-reproducible all-ranks form, for the 8-bit arm, and for the calibration pair `eager` vs `stock` (two
     implementations of the same stock layer that differ only in where SwiGLU rounds)."""
     from lcgemm import ops
     from lcgemm.model import DecoderConfig, RandomInitDecoder, compare_arms
@@ -1316,13 +1316,14 @@ def run_model(args, device):
     model = RandomInitDecoder(cfg, device)
     flush = torch.empty(FLUSH_BYTES, dtype=torch.int8, device=device)
     lengths = [int(t) for t in args.model_tokens.split(",")]
+    model.quantize()
     for tokens in lengths:
         info = model.install(tokens)
         prompts = [torch.randint(0, cfg.vocab, (tokens,),
                                  generator=torch.Generator().manual_seed(tokens + 7919 * j)).to(device)
                    for j in range(args.prompts)]
         ids = prompts[0]
-        times = {"stock": [], "rank7": [], "dense": []}
+        times = {"stock": [], "rank7": [], "dense": [], "fp8": []}
         for arm in times:
             for _ in range(max(1, args.warmup - 2)):
                 model.prefill(ids, arm=arm)
@@ -1333,8 +1334,8 @@ def run_model(args, device):
                 times[arm] += _event_times(lambda: model.prefill(ids, arm=arm), 1, 0, flush)
         ops.check_status()
         fused = model.calls["fused"] - before["fused"]
-        st, r7, dn = (statistics.median(times[a]) for a in ("stock", "rank7", "dense"))
-        pairs = {"rank7": [], "rank7_allranks": [], "eager": [], "dense": []}
+        st, r7, dn, f8 = (statistics.median(times[a]) for a in ("stock", "rank7", "dense", "fp8"))
+        pairs = {"rank7": [], "rank7_allranks": [], "eager": [], "dense": [], "fp8": []}
         repeat_equal = []
         for ids_j in prompts:
             ref = model.prefill(ids_j, arm="stock")
@@ -1344,6 +1345,10 @@ def run_model(args, device):
                 if arm == "rank7_allranks":
                     again = model.prefill(ids_j, arm=arm)
                     repeat_equal.append(bool(torch.equal(got[0], again[0]) and torch.equal(got[1], again[1])))
+        # mean log probability of the first prompt's tokens under each arm (uniform-random tokens on random
+        # weights: about -ln(vocab), equal in all arms up to what their MLPs change)
+        mean_logprob = {arm: float(model.prompt_logprobs(ids, arm=arm).logprob.double().mean())
+                        for arm in ("stock", "rank7", "dense", "fp8")}
         ops.check_status()
 
         def rates(rows):
@@ -1361,6 +1366,8 @@ def run_model(args, device):
             "model": "random-init dense decoder", "layers": cfg.layers, "hidden": cfg.hidden,
             "inter": cfg.inter, "heads": [cfg.q_heads, cfg.kv_heads, cfg.head_dim], "vocab": cfg.vocab,
             "tokens": tokens, "passes": args.steps, "stock_ms": st, "rank7_ms": r7, "dense_tcgen05_ms": dn,
+            "fp8_ms": f8, "fp8_speedup_pct": (st / f8 - 1.0) * 100.0, "prompt_mean_logprob": mean_logprob,
+            "agreement_fp8_vs_stock": rates(pairs["fp8"]),
             "speedup_pct": (st / r7 - 1.0) * 100.0, "speedup_vs_dense_tcgen05_pct": (dn / r7 - 1.0) * 100.0,
             "fused_calls": fused,
             "expected_fused_calls": args.steps * cfg.layers, "planes_gib": info["planes_gib"],

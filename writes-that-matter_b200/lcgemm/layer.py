@@ -1,4 +1,4 @@
-"""One dense-decoder MLP layer in three arms, for the single-layer configuration
+"""One dense-decoder MLP layer in four arms, for the single-layer configuration
 ``x -> RMSNorm -> gate_up -> SwiGLU -> down -> + residual`` and as the building block of the
 tensor-parallel form.
 
@@ -7,9 +7,11 @@ tensor-parallel form.
   plus the closing residual add;
 * :class:`DenseMlpLayer`  the stock layer (``lcgemm/integrate/qwen_patch.py:41-58``) on the
   dense tcgen05 GEMM of this library, or on cuBLAS through ``torch.matmul`` with
-  ``gemm="cublas"``: norm, GEMM, SwiGLU, GEMM, residual add.
+  ``gemm="cublas"``: norm, GEMM, SwiGLU, GEMM, residual add;
+* :class:`Fp8MlpLayer`  the stock layer with both GEMMs in 8 bits, a scale for each block of 128:
+  norm and SwiGLU quantise what they produce, so neither product's operand is ever written in bf16.
 
-Both keep the layer's output buffers and return views of them.
+All keep the layer's output buffers and return views of them.
 """
 from __future__ import annotations
 
@@ -103,6 +105,43 @@ class DenseMlpLayer:
     def forward(self, x, delta=None):
         d, h = self.chain(delta, x)
         return ops.add(h, d, out=self.out)
+
+    __call__ = forward
+    launches_per_forward = 5
+    accepts_no_delta = True
+
+
+class Fp8MlpLayer:
+    """The weights are quantised once, here.  Takes any number of rows up to ``tokens``, single tokens of
+    a decode step included: the product picks its form by the row count."""
+
+    def __init__(self, tokens: int, norm_weight, gate_up_weight, down_weight, eps: float = 1e-6):
+        two_i, hidden = gate_up_weight.shape
+        out_dim, inter = down_weight.shape
+        if two_i != 2 * inter:
+            raise ValueError("gate_up weight must have 2 * intermediate rows")
+        dev, bf = gate_up_weight.device, torch.bfloat16
+        self.eps, self.norm_weight, self.tokens = eps, norm_weight, tokens
+        self.w_gu, self.w_gu_scale = ops.quantize_fp8(gate_up_weight, block_rows=ops.FP8_BLOCK)
+        self.w_down, self.w_down_scale = ops.quantize_fp8(down_weight, block_rows=ops.FP8_BLOCK)
+        self.h = torch.empty((tokens, hidden), device=dev, dtype=bf)
+        self.z = torch.empty((tokens, two_i), device=dev, dtype=bf)
+        self.d = torch.empty((tokens, out_dim), device=dev, dtype=bf)
+        self.out = torch.empty((tokens, out_dim), device=dev, dtype=bf)
+
+    def chain(self, delta, residual):
+        m = residual.shape[0]
+        if m > self.tokens:
+            raise ValueError(f"the layer was built for at most {self.tokens} rows, got {m}")
+        q, scale, h = ops.add_rmsnorm_fp8(delta, residual, self.norm_weight, self.eps,
+                                          residual_out=None if delta is None else self.h[:m])
+        z = ops.gemm_fp8(q, scale, self.w_gu, self.w_gu_scale, out=self.z[:m])
+        q, scale = ops.swiglu_fp8(z)
+        return ops.gemm_fp8(q, scale, self.w_down, self.w_down_scale, out=self.d[:m]), h
+
+    def forward(self, x, delta=None):
+        d, h = self.chain(delta, x)
+        return ops.add(h, d, out=self.out[:x.shape[0]])
 
     __call__ = forward
     launches_per_forward = 5

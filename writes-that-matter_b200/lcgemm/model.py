@@ -18,7 +18,9 @@ Arms of :meth:`RandomInitDecoder.prefill`:
 ``"rank7_allranks"``  the same plans on the all-ranks schedule for both GEMMs: every C block
               has one writer and a fixed order of additions, so the result is reproducible bit
               for bit (slower: ``down`` then has fewer tiles than the GPU has CTA pairs);
-``"dense"``   the stock layer on this package's dense tcgen05 GEMM.
+``"dense"``   the stock layer on this package's dense tcgen05 GEMM;
+``"fp8"``     the stock layer with both GEMMs in 8 bits, a scale for each block of 128 (weights quantised
+              by :meth:`quantize`).
 
 The input norm of every layer uses the fused add + RMSNorm kernel in all arms.
 """
@@ -87,7 +89,7 @@ class RandomInitDecoder:
         self._plans = {}
         self._plans_det = {}
         self._dense = {}
-        self.calls = {"fused": 0, "reference": 0}
+        self.calls = {"fused": 0, "reference": 0, "fp8": 0}
 
     # ------------------------------------------------------------------ install
     def install(self, tokens: int) -> dict:
@@ -110,6 +112,16 @@ class RandomInitDecoder:
         return {"layers": cfg.layers, "tokens": tokens, "planes_gib": nbytes / 2 ** 30,
                 "describe": {"gate_up": gate.describe(), "down": down.describe()}}
 
+    def quantize(self) -> dict:
+        """8-bit MLP weights for every layer, for the ``"fp8"`` arm (any prompt length)."""
+        nbytes = 0
+        for layer in self.layers:
+            if "gate_up_fp8" not in layer:
+                layer["gate_up_fp8"] = ops.quantize_fp8(layer["gate_up"], block_rows=ops.FP8_BLOCK)
+                layer["down_fp8"] = ops.quantize_fp8(layer["down"], block_rows=ops.FP8_BLOCK)
+            nbytes += sum(t.numel() * t.element_size() for t in layer["gate_up_fp8"] + layer["down_fp8"])
+        return {"layers": self.cfg.layers, "fp8_gib": nbytes / 2 ** 30}
+
     # --------------------------------------------------------------------- MLP arms
     def _mlp(self, arm: str, layer: dict, delta, residual, ring):
         cfg = self.cfg
@@ -122,6 +134,13 @@ class RandomInitDecoder:
             gate(residual, delta, layer["post_norm"], cfg.eps, prepared_w=layer["gate_bw"],
                  residual_out=res_out)
             return down(prepared_w=layer["down_bw"]), res_out
+        if arm == "fp8":
+            self.calls["fp8"] += 1
+            res_out = ring[0]
+            ring.reverse()
+            q, scale, h = ops.add_rmsnorm_fp8(delta, residual, layer["post_norm"], cfg.eps, residual_out=res_out)
+            q, scale = ops.swiglu_fp8(ops.gemm_fp8(q, scale, *layer["gate_up_fp8"]))
+            return ops.gemm_fp8(q, scale, *layer["down_fp8"]), h
         self.calls["reference"] += 1
         if arm == "eager":
             h = (delta.float() + residual.float()).to(delta.dtype)
@@ -141,12 +160,14 @@ class RandomInitDecoder:
     @torch.no_grad()
     def prefill(self, token_ids: torch.Tensor, arm: str = "stock"):
         """Batch-1 prefill; returns (logits of the last position as fp32, final hidden state)."""
-        if arm not in ("stock", "eager", "rank7", "rank7_allranks", "dense"):
+        if arm not in ("stock", "eager", "rank7", "rank7_allranks", "dense", "fp8"):
             raise ValueError(f"unknown arm {arm!r}")
         cfg = self.cfg
         m = token_ids.shape[0]
         if arm in ("rank7", "rank7_allranks") and m not in self._plans:
             raise RuntimeError(f"install({m}) before a rank-7 prefill of {m} tokens")
+        if arm == "fp8" and any("gate_up_fp8" not in layer for layer in self.layers):
+            raise RuntimeError("quantize() before a prefill in the fp8 arm")
         pos = torch.arange(m, device=self.device, dtype=torch.float32)
         inv = 1.0 / (cfg.rope_theta ** (torch.arange(0, cfg.head_dim, 2, device=self.device,
                                                      dtype=torch.float32) / cfg.head_dim))
@@ -174,6 +195,21 @@ class RandomInitDecoder:
         final = _rmsnorm((hidden.float() + residual.float()).to(hidden.dtype), self.final_norm, cfg.eps)
         logits = F.linear(final[-1:], self.lm_head).float()[0]
         return logits, final
+
+
+    @torch.no_grad()
+    def prompt_logprobs(self, token_ids: torch.Tensor, arm: str = "stock", top: int = 0, rows: int = 4096):
+        """:class:`ops.TokenLogprobs` of every prompt token but the first, given those before it, with
+        the entropy at its position and the ``top`` likeliest tokens there: what an engine returns for prompt
+        log probabilities, the numbers the arms are compared by.  The head runs ``rows`` positions at a time."""
+        if token_ids.dim() != 1 or token_ids.shape[0] < 2:
+            raise ValueError(f"a prompt of at least two tokens, got {tuple(token_ids.shape)}")
+        if rows < 1:
+            raise ValueError(f"rows must be positive, got {rows}")
+        final = self.prefill(token_ids, arm=arm)[1][:-1]
+        parts = [ops.token_logprobs(F.linear(final[i:i + rows], self.lm_head), token_ids[1 + i:1 + i + rows], top=top)
+                 for i in range(0, final.shape[0], rows)]
+        return ops.TokenLogprobs(*(torch.cat(column) for column in zip(*parts)))
 
 
 LOGIT_STEP = 0.125      # one quantisation step of the log-probabilities (lcgemm/bench/prefill.py:180-183)
