@@ -53,6 +53,13 @@ __device__ __forceinline__ void regs_dec() {
 constexpr int kCodeProducer = 101, kCodeMmaAcc = 102, kCodeMmaFull = 103, kCodeEpilogue = 104;
 
 // ================================================================ many rows
+// A pair multiplies 256 rows of a by kBN rows of b; TMEM holds the sums of 512 / kBN blocks.  The
+// read-back walks these stages in a loop unrolled over four blocks, so that barriers, parities and TMEM
+// addresses are constants; the stages that the last K blocks of a tile leave over are only passed on.
+// (With the MMA issuer unrolled as well and more waits inlined, the loops did not fit the instruction
+// cache: 1054 us for 4096 x 34816 x 5120.  Four stages of 128 columns under a 256-wide tile, two MMAs to a slice of K, give
+// the read-back more slack but read a's tile from shared memory twice: 765 us where two of 256 take 695.)
+//
 // 12 warps: 0 TMA producer, 1 MMA issuer, 2 and 3 scales, 4-7 and 8-11 read-back: every warp one
 // TMEM lane quarter, each warpgroup half of the columns.
 template <int kBN>
@@ -64,6 +71,7 @@ struct Many {
   static constexpr int kCols = kBN / 2;                     // columns per read-back warpgroup
   static constexpr int kStoreBytes = 32 * 128;              // a warp's staged 32 x 64 bf16
   static constexpr int kGroup = 4;                          // K blocks whose scales travel together
+  static_assert(kGroup % kAcc == 0, "scales change between walks of the stages");
   static constexpr int kSlots = 4;
   static constexpr int kSlotFloats = kGroup * 2 * kTileRows;
   static constexpr int kSmemBytes = kStages * kStageBytes + 8 * kStoreBytes + kSlots * kSlotFloats * 4 + 256 + 1024;
@@ -187,6 +195,12 @@ k_gemm_fp8(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CU
         const uint64_t adesc0 = make_kmajor_sw128_desc(base);
         const uint64_t bdesc0 = make_kmajor_sw128_desc(base + kOperandBytes);
         uint32_t stage = 0, parity = 0, as = 0, acc_parity = 1;
+        auto next_stage = [&] {
+          if (++as == T::kAcc) {
+            as = 0;
+            acc_parity ^= 1u;
+          }
+        };
         for (int t = pair; t < p.num_tiles; t += num_pairs) {
           for (int kb = 0; kb < p.k_blocks; ++kb) {
             const uint64_t soff = static_cast<uint64_t>(stage * (T::kStageBytes >> 4));
@@ -203,14 +217,17 @@ k_gemm_fp8(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CU
               umma_commit<2>(empty_bar(stage));
             }
             __syncwarp();
-            if (++as == T::kAcc) {
-              as = 0;
-              acc_parity ^= 1u;
-            }
+            next_stage();
             if (++stage == T::kStages) {
               stage = 0;
               parity ^= 1u;
             }
+          }
+          while (as != 0) {          // every tile starts at stage 0
+            mbar_wait_inline(acc_empty_bar(as), acc_parity, ctl, kCodeMmaAcc);
+            if (elect_one()) umma_commit<2>(acc_full_bar(as));
+            __syncwarp();
+            next_stage();
           }
         }
       }
@@ -267,18 +284,20 @@ k_gemm_fp8(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CU
     const uint32_t lane_addr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + wg * T::kCols;
     const uint32_t buf = store_base + (warp - 4) * T::kStoreBytes;
     const float* my_scale = scales + wg * kTileRows + quarter * 32 + lane;
-    uint32_t as = 0, acc_parity = 0, slot = 0, slot_parity = 0;
+    uint32_t acc_parity = 0, slot = 0, slot_parity = 0;
     for (int t = pair; t < p.num_tiles; t += num_pairs) {
       uint64_t acc[T::kCols / 2];
 #pragma unroll
       for (int j = 0; j < T::kCols / 2; ++j) acc[j] = 0;
-      // Loads of 32 columns.  Each is issued before the one in front of it is used, across the stages
-      // of a tile too: the wait is for all of a warp's loads, so there is one in flight.
+      // Loads of 32 columns.  The wait is for all of a warp's loads, so there is one in flight: each is issued
+      // before the one in front of it is used, across the stages of a tile too.
       constexpr int kChunks = T::kCols / 32;
+      constexpr uint32_t kFlip = (T::kGroup / T::kAcc) & 1;     // whether a group leaves the stages' parity changed
+      uint32_t group_parity = acc_parity;
       uint32_t v[2][32];
-      mbar_wait_inline(acc_full_bar(as), acc_parity, ctl, kCodeEpilogue);
+      mbar_wait_inline(acc_full_bar(0), acc_parity, ctl, kCodeEpilogue);
       tcgen05_fence_after();
-      tmem_ld_32x32(lane_addr + as * kBN, v[0]);
+      tmem_ld_32x32(lane_addr, v[0]);
       for (int kb0 = 0; kb0 < p.k_blocks; kb0 += T::kGroup) {
         mbar_wait_inline(scale_full_bar(slot), slot_parity, ctl, kCodeEpilogue);
         float sc[T::kGroup];
@@ -294,6 +313,8 @@ k_gemm_fp8(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CU
         for (int i = 0; i < T::kGroup; ++i) {
           if (kb0 + i < p.k_blocks) {
             const uint64_t s2 = pack_f32x2(__float_as_uint(sc[i]), __float_as_uint(sc[i]));
+            const uint32_t as = i % T::kAcc, next = (i + 1) % T::kAcc;
+            const uint32_t next_parity = group_parity ^ (((i + 1) / T::kAcc) & 1);
 #pragma unroll
             for (int c = 0; c < kChunks; ++c) {
               tmem_ld_wait(v[c & 1]);
@@ -303,14 +324,10 @@ k_gemm_fp8(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CU
                 tcgen05_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive_cluster_relaxed(acc_empty_leader + 8u * as);
-                if (++as == T::kAcc) {
-                  as = 0;
-                  acc_parity ^= 1u;
-                }
                 if (kb0 + i + 1 < p.k_blocks) {
-                  mbar_wait_inline(acc_full_bar(as), acc_parity, ctl, kCodeEpilogue);
+                  mbar_wait_inline(acc_full_bar(next), next_parity, ctl, kCodeEpilogue);
                   tcgen05_fence_after();
-                  tmem_ld_32x32(lane_addr + as * kBN, v[0]);
+                  tmem_ld_32x32(lane_addr + next * kBN, v[0]);
                 }
               }
 #pragma unroll
@@ -319,7 +336,15 @@ k_gemm_fp8(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CU
             }
           }
         }
+        group_parity ^= kFlip;
       }
+      const int last_walk = (p.k_blocks - 1) / T::kAcc;
+      for (int s = (p.k_blocks - 1) % T::kAcc + 1; s < T::kAcc; ++s) {      // passed on (see the issuer)
+        mbar_wait_inline(acc_full_bar(s), acc_parity ^ (last_walk & 1), ctl, kCodeEpilogue);
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster_relaxed(acc_empty_leader + 8u * s);
+      }
+      acc_parity ^= (last_walk + 1) & 1;
       // bf16, 64 columns at a time through this warp's staging buffer
       int tm, tn;
       tile_at(t, tm, tn);
