@@ -82,4 +82,8 @@ def test_logprobs_check_their_arguments(native_lib):
         assert bad(i, None) == nat.ERR_BAD_ARG
     assert bad(1, 3) == bad(4, 99) == bad(6, 2) == bad(7, 33) == bad(7, -1) == nat.ERR_BAD_ARG
     assert bad(2, 0) == bad(3, 0) == nat.ERR_UNSUPPORTED_SHAPE
+    assert bad(3, (1 << 20) + 1) == bad(2, 1 << 31) == nat.ERR_UNSUPPORTED_SHAPE
+    assert bad(0, P + 1) == nat.ERR_MISALIGNED
+    assert native_lib.lcg_token_logprobs(P + 2, nat.DTYPE_FP32, 4, 100, 100, P, 8, 0, P, P, None, None,
+                                         None) == nat.ERR_MISALIGNED
     assert native_lib.lcg_token_logprobs(P, nat.DTYPE_BF16, 4, 3, 3, P, 8, 4, P, P, P, P, None) == nat.ERR_BAD_ARG

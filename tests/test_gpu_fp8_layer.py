@@ -163,3 +163,101 @@ def test_decoder_arm_and_prompt_logprobs():
         assert bool((got.top_logprobs[:, :-1] >= got.top_logprobs[:, 1:]).all())
     with pytest.raises(ValueError):
         model.prompt_logprobs(tokens[:1])
+
+
+def test_offsets_past_32_bits():
+    """Matrices of more than 2^31 elements: the last rows are where they belong."""
+    from lcgemm import ops
+
+    # quantiser and log probabilities: 2^31 bf16 values and some
+    v, m = 131075, 16400
+    big = torch.zeros((m, v), dtype=torch.bfloat16, device="cuda")
+    tail = seeded((3, v), 41, 2.0)
+    big[-3:] = tail
+    ids = torch.full((m,), 7, device="cuda")
+    got = ops.token_logprobs(big, ids, top=4)
+    want = ops.token_logprobs(tail, ids[:3], top=4)
+    # 3 rows are split over clusters and 16400 are not, so the sums associate differently: each is within
+    # (V / 256 + 64) 2^-24 + 2^-21 of the exact S and T (tests/test_gpu_logprobs.py), twice that of the other
+    rel = 2 * ((v / 256 + 64) * 2.0 ** -24 + 2.0 ** -21)
+    assert torch.equal(got.top_ids[-3:], want.top_ids)
+    assert bool(((got.logprob[-3:] - want.logprob).abs() <= rel + 2.0 ** -21 * want.logprob.abs()).all())
+    assert bool(((got.top_logprobs[-3:] - want.top_logprobs).abs() <= rel + 2.0 ** -21 * want.top_logprobs.abs()).all())
+    assert bool(((got.entropy[-3:] - want.entropy).abs() <= rel * (2 + want.entropy)).all())
+    assert torch.equal(got.top_ids[0].cpu(), torch.arange(4))
+    q, s = ops.quantize_fp8(big)
+    want_q, want_s = ops.quantize_fp8(tail)
+    assert torch.equal(q[-3:].view(torch.uint8), want_q.view(torch.uint8)) and torch.equal(s[-3:], want_s)
+    del big, q, s, got
+    # the product: an output of 2^31 values and some, for many rows; for few rows a weight of as many
+    m, n = 65600, 32776
+    a, sa = ops.quantize_fp8(seeded((m, 32), 42))
+    b, sb = ops.quantize_fp8(seeded((n, 32), 43), block_rows=128)
+    out = ops.gemm_fp8(a, sa, b, sb)
+    assert torch.equal(out[-300:], ops.gemm_fp8(a[-300:], sa[-300:], b, sb))
+    del out
+    n, k = 131200, 16400
+    w = torch.zeros((n, k), dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn)
+    last, last_s = ops.quantize_fp8(seeded((128, k), 44), block_rows=128)
+    w[-128:].view(torch.uint8).copy_(last.view(torch.uint8))
+    ws = torch.ones((n // 128, -(-k // 128)), device="cuda")
+    ws[-1] = last_s[0]
+    x, sx = ops.quantize_fp8(seeded((2, k), 45))
+    got = ops.gemm_fp8(x, sx, w, ws)
+    ops.check_status()
+    want = decode(x, sx, 1) @ decode(last, last_s, 128).T
+    size = decode(x, sx, 1).abs() @ decode(last, last_s, 128).abs().T
+    assert bool(((got[:, -128:].double().cpu() - want).abs() <= 2.0 ** -8 * want.abs() + (128 + 129 + 2) * 2.0 ** -23 * size).all())
+    assert not bool(got[:, :-128].any())
+
+
+def test_first_product_inside_a_capture_is_refused():
+    from lcgemm import ops
+
+    q, s = ops.quantize_fp8(seeded((4, 256), 1))
+    w, ws = ops.quantize_fp8(seeded((64, 256), 2), block_rows=128)
+    word = ops._STATUS.pop(q.device, None)
+    try:
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with pytest.raises(RuntimeError, match="before a graph capture"):
+            with torch.cuda.graph(graph):
+                ops.gemm_fp8(q, s, w, ws)
+    finally:
+        if word is not None:
+            ops._STATUS[q.device] = word
+    torch.cuda.synchronize()
+    assert torch.isfinite(ops.gemm_fp8(q, s, w, ws)).all()
+
+
+def test_tensors_on_another_device():
+    from lcgemm import ops
+
+    if torch.cuda.device_count() < 2:
+        pytest.skip("needs two devices")
+    x = seeded((5, 256), 1)
+    other = x.to("cuda:1")
+    assert torch.cuda.current_device() == 0
+    q, s = ops.quantize_fp8(other)
+    w, ws = ops.quantize_fp8(seeded((64, 256), 2).to("cuda:1"), block_rows=128)
+    c = ops.gemm_fp8(q, s, w, ws)
+    lp = ops.token_logprobs(c, torch.zeros(5, dtype=torch.int64, device="cuda:1"), top=3)
+    torch.cuda.synchronize(1)
+    assert c.device == lp.logprob.device == other.device and torch.cuda.current_device() == 0
+    q0, s0 = ops.quantize_fp8(x)
+    assert torch.equal(q.cpu().view(torch.uint8), q0.cpu().view(torch.uint8)) and torch.equal(s.cpu(), s0.cpu())
+    with pytest.raises(ValueError, match="one device"):
+        ops.gemm_fp8(q0, s0, w, ws)
+
+
+def test_scales_of_stride_zero():
+    """One scale for a whole matrix is a tensor of stride 0."""
+    from lcgemm import ops
+
+    for m in (4, 300):
+        q, _ = ops.quantize_fp8(seeded((m, 300), 1))
+        w, _ = ops.quantize_fp8(seeded((200, 300), 2), block_rows=128)
+        one = torch.full((1, 1), 0.25, device="cuda")
+        got = ops.gemm_fp8(q, one.expand(m, 3), w, one.expand(2, 3))
+        want = ops.gemm_fp8(q, one.repeat(m, 3), w, one.repeat(2, 3))
+        assert torch.equal(got, want)

@@ -195,12 +195,5 @@ def stream_ptr() -> int:
     return torch.cuda.current_stream().cuda_stream
 
 
-def raw_stream(device: int) -> int:
-    """Handle of the current stream of a device, without the Python object around it (3 us less a call)."""
-    import torch
-
-    return torch._C._cuda_getCurrentRawStream(device)
-
-
 def ptr(t) -> int:
     return t.data_ptr() if t is not None else 0

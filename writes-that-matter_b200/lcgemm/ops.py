@@ -13,7 +13,7 @@ from typing import NamedTuple
 import torch
 
 from . import _native as nat
-from ._native import NativeScheme, check, lib, ptr, raw_stream, stream_ptr
+from ._native import NativeScheme, check, lib, ptr, stream_ptr
 
 BF16 = torch.bfloat16
 E4M3 = torch.float8_e4m3fn
@@ -459,6 +459,7 @@ def add(a: torch.Tensor, b: torch.Tensor, out: torch.Tensor | None = None) -> to
 # short: one allocation call per output, the raw stream handle, no context managers on the usual path.
 _current_device = torch.cuda.current_device
 _empty = torch.empty_strided
+_raw_stream = torch._C._cuda_getCurrentRawStream      # the handle, without the Python object around it
 _F32 = torch.float32
 
 
@@ -507,13 +508,15 @@ def quantize_fp8(x: torch.Tensor, block_rows: int = 1):
     device = x.device
     q = _codes(m, k, device)
     if block_rows == 1:
-        scale = _row_scales(m, k, device)
+        scale, s_row, s_blk = _row_scales(m, k, device), 1, max(m, 1)
     else:
-        scale = torch.empty((-(-m // FP8_BLOCK), -(-k // FP8_BLOCK)), dtype=_F32, device=device)
+        s_row, s_blk = -(-k // FP8_BLOCK), 1
+        scale = _empty((-(-m // FP8_BLOCK), s_row), (s_row, 1), dtype=_F32, device=device)
     if m > 0:
-        s_row, s_blk = scale.stride()
-        check(lib().lcg_quantize_fp8(x.data_ptr(), m, k, x.stride(0), block_rows, q.data_ptr(), q.stride(0),
-                                     scale.data_ptr(), s_row, s_blk, raw_stream(dev)))
+        code = lib().lcg_quantize_fp8(x.data_ptr(), m, k, x.stride(0), block_rows, q.data_ptr(), (k + 15) // 16 * 16,
+                                      scale.data_ptr(), s_row, s_blk, _raw_stream(dev))
+        if code:
+            check(code)
     return q, scale
 
 
@@ -522,9 +525,9 @@ def add_rmsnorm_fp8(delta, residual, norm_weight, eps: float, residual_out=None)
     quantised by rows from its fp32 value.  Without a ``delta`` the third value is ``residual`` itself
     and nothing is stored for it.  ``residual_out`` may be ``residual``."""
     _need(residual, "residual"), _need(norm_weight, "norm weight")
-    if residual.dim() != 2 or not residual.is_contiguous():
-        raise ValueError(f"residual must be a contiguous matrix, got {tuple(residual.shape)}")
     shape = residual.shape
+    if len(shape) != 2 or not residual.is_contiguous():
+        raise ValueError(f"residual must be a contiguous matrix, got {tuple(shape)}")
     m, k = shape
     if norm_weight.shape != (k,) or not norm_weight.is_contiguous():
         raise ValueError(f"norm weight must be a contiguous ({k},) tensor")
@@ -550,18 +553,20 @@ def add_rmsnorm_fp8(delta, residual, norm_weight, eps: float, residual_out=None)
     device = residual.device
     q, scale = _codes(m, k, device), _row_scales(m, k, device)
     if m > 0:
-        s_row, s_blk = scale.stride()
-        check(lib().lcg_add_rmsnorm_fp8(d_ptr, residual.data_ptr(), norm_weight.data_ptr(), m, k, eps, h_ptr,
-                                        q.data_ptr(), q.stride(0), scale.data_ptr(), s_row, s_blk, raw_stream(dev)))
+        code = lib().lcg_add_rmsnorm_fp8(d_ptr, residual.data_ptr(), norm_weight.data_ptr(), m, k, float(eps), h_ptr,
+                                         q.data_ptr(), (k + 15) // 16 * 16, scale.data_ptr(), 1, m, _raw_stream(dev))
+        if code:
+            check(code)
     return q, scale, residual if delta is None else residual_out
 
 
 def swiglu_fp8(z: torch.Tensor):
     """``(codes, scales)`` of ``silu(z[:, :I]) * z[:, I:]``, quantised by rows from its fp32 value."""
     _need(z, "z")
-    if z.dim() != 2 or z.shape[1] % 2 != 0:
-        raise ValueError(f"z must be an (M, 2 * I) matrix, got {tuple(z.shape)}")
-    m, inter = z.shape[0], z.shape[1] // 2
+    shape = z.shape
+    if len(shape) != 2 or shape[1] % 2 != 0:
+        raise ValueError(f"z must be an (M, 2 * I) matrix, got {tuple(shape)}")
+    m, inter = shape[0], shape[1] // 2
     dev = z.get_device()
     if dev != _current_device():
         with torch.cuda.device(dev):
@@ -569,9 +574,10 @@ def swiglu_fp8(z: torch.Tensor):
     device = z.device
     q, scale = _codes(m, inter, device), _row_scales(m, inter, device)
     if m > 0:
-        s_row, s_blk = scale.stride()
-        check(lib().lcg_swiglu_fp8(z.data_ptr(), m, inter, z.stride(0), q.data_ptr(), q.stride(0), scale.data_ptr(),
-                                   s_row, s_blk, raw_stream(dev)))
+        code = lib().lcg_swiglu_fp8(z.data_ptr(), m, inter, z.stride(0), q.data_ptr(), (inter + 15) // 16 * 16,
+                                    scale.data_ptr(), 1, m, _raw_stream(dev))
+        if code:
+            check(code)
     return q, scale
 
 
@@ -613,10 +619,15 @@ def gemm_fp8(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: t
     if out is None:
         out = _empty((m, n), (n, 1), dtype=BF16, device=a.device) if n % 8 == 0 else _padded_out(m, n, a.device)
     if m > 0:
+        if a.device not in _STATUS and torch.cuda.is_current_stream_capturing():
+            # the word would belong to the graph and be cleared only by its replays
+            raise RuntimeError("the first product on a device must come before a graph capture: call it once")
         (as_row, as_blk), (bs_row, bs_blk) = a_scale.stride(), b_scale.stride()
-        check(lib().lcg_gemm_fp8(a.data_ptr(), lda, a_scale.data_ptr(), as_row, as_blk, b.data_ptr(), ldb,
-                                 b_scale.data_ptr(), bs_row, bs_blk, out.data_ptr(), out.stride(0), m, n, k,
-                                 status_word(a.device).data_ptr(), raw_stream(dev)))
+        code = lib().lcg_gemm_fp8(a.data_ptr(), lda, a_scale.data_ptr(), as_row, as_blk, b.data_ptr(), ldb,
+                                  b_scale.data_ptr(), bs_row, bs_blk, out.data_ptr(), out.stride(0), m, n, k,
+                                  status_word(a.device).data_ptr(), _raw_stream(dev))
+        if code:
+            check(code)
     return out
 
 
@@ -641,13 +652,15 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
     kind = _LOGIT_TYPES.get(logits.dtype)
     if kind is None:
         raise ValueError(f"logits must be bfloat16, float16 or float32, got {logits.dtype}")
-    if logits.dim() != 2 or (logits.stride(1) != 1 and logits.shape[1] > 1):
-        raise ValueError(f"logits must be a row-major (M, V) matrix, got {tuple(logits.shape)}")
-    m, v = logits.shape
+    shape = logits.shape
+    if len(shape) != 2 or (logits.stride(1) != 1 and shape[1] > 1):
+        raise ValueError(f"logits must be a row-major (M, V) matrix, got {tuple(shape)}")
+    m, v = shape
     if tokens.dtype not in (torch.int64, torch.int32) or tokens.shape != (m,):
         raise ValueError(f"tokens must be ({m},) of int64 or int32, got {tuple(tokens.shape)} of {tokens.dtype}")
     if v < 1:
         raise ValueError("logits have no columns")
+    top = int(top)
     if not 0 <= top <= min(MAX_TOP, v):
         raise ValueError(f"top must be between 0 and {min(MAX_TOP, v)}, got {top}")
     dev = logits.get_device()
@@ -662,7 +675,9 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
     top_lp = _empty((m, top), (pitch, 1), dtype=_F32, device=device)
     top_ids = _empty((m, top), (pitch, 1), dtype=torch.int64, device=device)
     if m > 0:
-        check(lib().lcg_token_logprobs(logits.data_ptr(), kind, m, v, logits.stride(0), tokens.data_ptr(),
-                                       tokens.element_size(), top, logprob.data_ptr(), entropy.data_ptr(),
-                                       top_lp.data_ptr(), top_ids.data_ptr(), raw_stream(dev)))
+        code = lib().lcg_token_logprobs(logits.data_ptr(), kind, m, v, logits.stride(0), tokens.data_ptr(),
+                                        tokens.element_size(), top, logprob.data_ptr(), entropy.data_ptr(),
+                                        top_lp.data_ptr(), top_ids.data_ptr(), _raw_stream(dev))
+        if code:
+            check(code)
     return TokenLogprobs(logprob, entropy, top_lp, top_ids)
