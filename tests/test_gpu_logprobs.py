@@ -159,3 +159,27 @@ def test_empty_batch_and_refusals():
                  lambda: ops.token_logprobs(x[0].expand(4, 64), t)):
         with pytest.raises(ValueError):
             call()
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_many_long_rows(kind):
+    """Enough rows that each is one CTA's: random, tied, rising, masked and bad ones among them, at an odd pitch."""
+    from lcgemm import ops
+
+    m, v, top = 604, 17001, 20
+    g = torch.Generator().manual_seed(3)
+    big = (torch.randn((m, v + 2), generator=g) * 3).to(TYPES[kind])
+    big[1] = 0.0
+    big[2] = torch.arange(v + 2).float() / v * 20
+    big[3, v // 3:] = -math.inf
+    big[4, 1:] = torch.finfo(TYPES[kind]).min
+    big[5] = (torch.arange(v + 2) // 7 % 3).float()
+    tokens = torch.randint(0, v, (m,), generator=g)
+    dev = big.cuda()
+    got = check(big[:, 1:1 + v], tokens, top, dev[:, 1:1 + v])
+    view = dev[:, 1:1 + v]
+    dev[7, 100], dev[8] = math.nan, -math.inf
+    bad = ops.token_logprobs(view, tokens.cuda(), top=top)
+    assert bool(bad.logprob[7:9].isnan().all()) and bool(bad.top_logprobs[7:9].isnan().all())
+    keep = [i for i in range(m) if i not in (7, 8)]
+    assert all(torch.equal(a[keep], b[keep]) for a, b in zip(bad, got))

@@ -333,12 +333,14 @@ __device__ void select(const uint32_t* keys, int n, int k, uint32_t* out, Select
   if (found <= kPick) {
     if (tid >= found && tid < ((found + 7) & ~7)) sc.pick[tid] = 0;
     __syncthreads();
-    const uint64_t e = tid / 2 < found ? sc.pick[tid / 2] : 0;
-    int place = place_of<2>(sc.pick, found, 2 * (tid & 1), e);
-    place += __shfl_xor_sync(0xffffffffu, place, 1);
-    if (e != 0 && place < k && (tid & 1) == 0) {
-      out[place] = entry_id(e);
-      if (place == k - 1) sc.least = entry_key(e);
+    if (warp * 16 < found) {
+      const uint64_t e = tid / 2 < found ? sc.pick[tid / 2] : 0;
+      int place = place_of<2>(sc.pick, found, 2 * (tid & 1), e);
+      place += __shfl_xor_sync(0xffffffffu, place, 1);
+      if (e != 0 && place < k && (tid & 1) == 0) {
+        out[place] = entry_id(e);
+        if (place == k - 1) sc.least = entry_key(e);
+      }
     }
   } else if (warp == 0) {
     search<kBits>(keys, n, k, out, sc);
@@ -519,6 +521,7 @@ k_token_logprobs(const __grid_constant__ Params p) {
     // No value below the least of the chosen maxima is among the best: there are `want` that are not.
     // (Where all segments are chosen there is no such bound.)
     const uint32_t least = n > want ? s_select.least : 0u;
+    const float least_value = least == 0u ? -CUDART_INF_F : key_value<T>(least);
     auto id_of = [&](int run, int e) { return ((seg0 + static_cast<int>(s_run[run >> 5])) * 32 + (run & 31)) * kN - r.head + e; };
     if (n > want || last - first <= kMaxCands) {
       uint4 q[kMaxTop / kWarps];
@@ -536,9 +539,19 @@ k_token_logprobs(const __grid_constant__ Params p) {
         float f[kN];
         Vec<T>::unpack(q[u], f);
         uint32_t in = 0;
+        if (least_value > -CUDART_INF_F) {          // few lanes hold a candidate: values compare faster than keys
+#pragma unroll
+          for (int e = 0; e < kN; ++e)
+            if (f[e] >= least_value) in |= 1u << e;
+          if (__ballot_sync(0xffffffffu, in != 0) == 0u) continue;
+        } else {                                     // a NaN ranks with -inf
+#pragma unroll
+          for (int e = 0; e < kN; ++e)
+            if (order_key<T>(f[e]) >= least) in |= 1u << e;
+        }
 #pragma unroll
         for (int e = 0; e < kN; ++e)
-          if (order_key<T>(f[e]) >= least && id0 + e >= 0 && id0 + e < r.V) in |= 1u << e;
+          if (id0 + e < 0 || id0 + e >= r.V) in &= ~(1u << e);
         append(in, [&](int e) { return order_key<T>(f[e]); }, id0);
       }
     } else if (tid == 0) {
