@@ -39,7 +39,7 @@ __device__ __forceinline__ uint32_t amax_bits8(const uint4& q) {
 }
 __device__ __forceinline__ float max3_abs(float a, float b, float c) {      // a NaN stays one
   float r;
-  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(fabsf(a)), "f"(fabsf(b)), "f"(fabsf(c)));
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
 __device__ __forceinline__ uint32_t amax_bits8(const float (&f)[8]) {
@@ -309,7 +309,16 @@ k_add_rmsnorm_fp8(const __nv_bfloat16* __restrict__ delta, const __nv_bfloat16* 
   }
 }
 
-// silu(g) * u quantised from its fp32 value; silu(g) = g / (1 + e^-g).  A 16-lane group to a block of the
+// silu(g) = g / (1 + e^-g) with the hardware's base-2 exponential and reciprocal, subnormals to 0: where
+// e^-g passes 2^126 the value is below 2^-119, under every block's floor.
+__device__ __forceinline__ float silu(float g) {
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * -1.4426950408889634f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+  return g * r;
+}
+
+// silu(g) * u quantised from its fp32 value.  A 16-lane group to a block of the
 // result, kGluUnroll blocks in turn with all their loads in flight (4096 x 17408: one at a time 82 us).
 constexpr int kGluUnroll = 2;
 __global__ void __launch_bounds__(256)
@@ -338,7 +347,7 @@ k_swiglu_fp8(const __nv_bfloat16* __restrict__ z, const Walk w, int inter, int64
     unpack8(gv[j], gf);
     unpack8(uv[j], uf);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) gf[e] = __fdividef(gf[e], 1.0f + __expf(-gf[e])) * uf[e];
+    for (int e = 0; e < 8; ++e) gf[e] = silu(gf[e]) * uf[e];
     const float a = __uint_as_float(block_max16(amax_bits8(gf)));
     float scale;
     const float inv = inverse_and_scale(a, scale);
