@@ -319,8 +319,8 @@ __device__ __forceinline__ float silu(float g) {
 }
 
 // silu(g) * u quantised from its fp32 value.  A 16-lane group to a block of the
-// result, kGluUnroll blocks in turn with all their loads in flight (4096 x 17408: one at a time 82 us).
-constexpr int kGluUnroll = 2;
+// result, kGluUnroll blocks in turn with all their loads in flight (4096 x 17408: 72, 68 and 64 us for one, two and four).
+constexpr int kGluUnroll = 4;
 __global__ void __launch_bounds__(256)
 k_swiglu_fp8(const __nv_bfloat16* __restrict__ z, const Walk w, int inter, int64_t ldz,
              uint8_t* __restrict__ q, int64_t ldq, ScaleOut sc) {
