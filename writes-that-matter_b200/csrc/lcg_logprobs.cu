@@ -500,24 +500,14 @@ k_token_logprobs(const __grid_constant__ Params p) {
       if (tid < n) s_run[tid] = tid;
       __syncthreads();
     }
-    // A warp's candidates, bit e of `in` for value e of a lane's vector, appended together.
-    auto append = [&](uint32_t in, const auto& key_of, int id0) {
-      if (__ballot_sync(0xffffffffu, in != 0) == 0u) return;
-      int sum = __popc(in);
-#pragma unroll
-      for (int o = 1; o < 32; o *= 2) {
-        const int up = __shfl_up_sync(0xffffffffu, sum, o);
-        if (lane >= o) sum += up;
-      }
-      int at = 0;
-      if (lane == 31) at = atomicAdd(&s_count, sum);
-      at = __shfl_sync(0xffffffffu, at, 31) + sum - __popc(in);
-#pragma unroll
-      for (int e = 0; e < kN; ++e) {
-        if (in & (1u << e)) {
-          if (at < kMaxCands) s_cand[at] = entry(key_of(e), static_cast<uint32_t>(id0 + e));
-          ++at;
-        }
+    // Candidates: value e of the vector at id0 for each bit e of `in`.  They are few, so each takes its place by
+    // itself and is read again (from L1) rather than picked out of registers.
+    auto append = [&](uint32_t in, int id0) {
+      while (in != 0u) {
+        const int id = id0 + __ffs(in) - 1;
+        in &= in - 1u;
+        const int at = atomicAdd(&s_count, 1);
+        if (at < kMaxCands) s_cand[at] = entry(order_key<T>(to_float(r.x[id])), static_cast<uint32_t>(id));
       }
     };
     // No value below the least of the chosen maxima is among the best: there are `want` that are not.
@@ -545,16 +535,14 @@ k_token_logprobs(const __grid_constant__ Params p) {
 #pragma unroll
           for (int e = 0; e < kN; ++e)
             if (f[e] >= least_value) in |= 1u << e;
-          if (__ballot_sync(0xffffffffu, in != 0) == 0u) continue;
         } else {                                     // a NaN ranks with -inf
 #pragma unroll
           for (int e = 0; e < kN; ++e)
             if (order_key<T>(f[e]) >= least) in |= 1u << e;
         }
-#pragma unroll
-        for (int e = 0; e < kN; ++e)
-          if (id0 + e < 0 || id0 + e >= r.V) in &= ~(1u << e);
-        append(in, [&](int e) { return order_key<T>(f[e]); }, id0);
+        if (id0 < 0) in &= 0xffffffffu << -id0;                     // the row's own values only
+        if (id0 + kN > r.V) in &= id0 < r.V ? (1u << (r.V - id0)) - 1u : 0u;
+        append(in, id0);
       }
     } else if (tid == 0) {
       s_count = kMaxCands + 1;
@@ -599,7 +587,7 @@ k_token_logprobs(const __grid_constant__ Params p) {
       const int at = tid / kN;
       const int id = at < vecs ? id_of(static_cast<int>(s_vec[at]), tid % kN) : -1;
       const uint32_t key = id >= 0 && id < r.V ? order_key<T>(to_float(r.x[id])) : 0u;
-      append(key != 0u && key >= least_of_vecs ? 1u : 0u, [&](int) { return key; }, id);
+      append(key != 0u && key >= least_of_vecs ? 1u : 0u, id);
       __syncthreads();
     }
     const int cands = s_count;
