@@ -18,7 +18,7 @@
 //
 // Many rows: 4096 x 151936 bf16 without alternatives run at HBM's rate (203 us, 190 at the copy rate; 66
 // instructions to a warp's 512 bytes, the exponential unit at 2/3 of its rate); 20 alternatives add
-// 11000 instructions a row, which no longer fit beside the pass (260 us).  One row is bound by the
+// 9300 instructions a row, which no longer fit beside the pass (239 us).  One row is bound by the
 // latency of the selection.  A row is one CTA's, or a cluster's of up to eight when there
 // are too few rows to fill the GPU; the CTAs' parts are joined through distributed shared memory in
 // rank order, so the result does not depend on timing.
@@ -722,10 +722,15 @@ extern "C" int lcg_token_logprobs(const void* logits, int dtype, int64_t M, int6
   p.entropy = entropy;
   p.top_logprobs = top_logprobs;
   p.top_ids = top_ids;
-  // CTAs to a row: enough to give every SM four CTAs, each with at least 16 segments (two loads a warp).
+  // CTAs to a row, each with at least 16 segments (two loads a warp).
   const int64_t segments = (V * static_cast<int64_t>(width) + 511) / 512;
+  // The cluster grows while the grid has fewer than two CTAs an SM, so it ends below four.  Past that the
+  // join and the choice in every CTA cost more than the shorter pass saves.  Against growing while there
+  // are fewer than four, at 151936 bf16 with 20 alternatives: 100 rows 19.5 us against 27.8, 200 rows
+  // 27.4 / 36.1, 500 rows 43.9 / 57.8; 333 x 50257 fp32 22.0 / 23.1.  Fewer than one: 100 rows 22.1,
+  // 200 rows 31.5.
   p.cluster = 1;
-  while (p.cluster < kMaxCluster && M * p.cluster < 4 * sm_count() && segments / (2 * p.cluster) >= 16) p.cluster *= 2;
+  while (p.cluster < kMaxCluster && M * p.cluster < 2 * sm_count() && segments / (2 * p.cluster) >= 16) p.cluster *= 2;
   auto st = static_cast<cudaStream_t>(stream);
   if (dtype == LCG_DTYPE_BF16) return run<__nv_bfloat16>(p, M, st);
   if (dtype == LCG_DTYPE_FP16) return run<__half>(p, M, st);
