@@ -7,6 +7,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "lcg_wait.h"
+
 namespace lcg {
 
 // ---------------------------------------------------------------- addressing
@@ -152,21 +154,11 @@ __device__ __forceinline__ void mbar_wait(uint32_t bar, uint32_t parity, const W
 }
 
 // The same without a call: for warps whose registers are full of accumulators, which a call's
-// register convention would move about.
-__device__ __forceinline__ void mbar_wait_inline(uint32_t bar, uint32_t parity, const WaitCtl& ctl, int code) {
-  uint64_t t0 = 0;
-  // the timer is read once in 64 tries: reading it takes longer than most waits
-  for (uint32_t tries = 1; !mbar_try_wait(bar, parity); ++tries) {
-    if ((tries & 63u) != 0) continue;
-    if (*ctl.abort_flag) return;
-    const uint64_t now = globaltimer_ns();
-    if (t0 == 0) t0 = now;
-    if (now - t0 > ctl.limit_ns) {
-      *ctl.abort_flag = 1u;
-      if (ctl.status != nullptr) atomicCAS(ctl.status, 0, code);
-      return;
-    }
-  }
+// register convention would move about.  Whether the wait was met.
+__device__ __forceinline__ bool mbar_wait_inline(uint32_t bar, uint32_t parity, const WaitCtl& ctl, int code) {
+  return bounded_wait(ctl.abort_flag, ctl.limit_ns, [&] { return mbar_try_wait(bar, parity); },
+                      [] { return globaltimer_ns(); },
+                      [&] { if (ctl.status != nullptr) atomicCAS(ctl.status, 0, code); });
 }
 
 // Bounded wait on a monotonically increasing shared-memory counter.
