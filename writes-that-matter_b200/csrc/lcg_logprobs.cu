@@ -662,6 +662,7 @@ k_token_logprobs(const __grid_constant__ Params p) {
       p.top_logprobs[row * p.top + tid] = (key_value<T>(entry_key(e)) - a.m) - lse;
     }
   }
+  __syncwarp();              // the cluster barriers are for whole warps
   if (p.cluster > 1) {       // nobody leaves while its part is being read
     cluster_arrive();
     cluster_wait();
