@@ -1,4 +1,4 @@
-"""The bounded wait of the 8-bit products (csrc/lcg_wait.h) compiled for the host, with a clock and a barrier of its own."""
+"""The bounded wait of the 8-bit products and the end of their rings (csrc/lcg_wait.h) compiled for the host, with a clock and a barrier of its own."""
 import shutil
 import subprocess
 
@@ -39,6 +39,29 @@ int main() {
   lcg::bounded_wait(&late.flag, 1500000000ull, [&] { if (++late.tries == 5) late.flag = 1; return false; },
                     [&] { return late.clock; }, [&] { ++late.reports; });
   std::printf("%llu %d\n", (unsigned long long)late.tries, late.reports);
+
+  // A ring of `stages` filled `fills` times.  The releases land late, each when a wait asks for it; a wait for
+  // parity p is met while the number of releases that landed in its stage is of the other parity.
+  int left = 0, stuck = 0;
+  for (uint32_t stages = 4; stages <= 7; ++stages) {
+    for (int fills = 1; fills < 40; ++fills) {
+      int landed[8] = {}, pending[8] = {};
+      auto wait = [&](uint32_t s, uint32_t p) {
+        if ((landed[s] & 1) != (int)p) return;
+        if (pending[s] == 0) ++stuck;
+        else --pending[s], ++landed[s];
+      };
+      uint32_t stage = 0, parity = 1;
+      for (int i = 0; i < fills; ++i) {
+        wait(stage, parity);
+        ++pending[stage];
+        if (++stage == stages) stage = 0, parity ^= 1u;
+      }
+      lcg::drain_ring(stages, stage, parity, wait);
+      for (int p : pending) left += p;
+    }
+  }
+  std::printf("%d %d\n", left, stuck);
 }
 """
 
@@ -68,3 +91,7 @@ def test_a_wait_that_is_not_met_gives_up_after_its_limit(lines):
 def test_once_one_has_run_out_every_later_wait_returns_at_once(lines):
     assert lines[2] == [5000, 1, 0]          # one try each, no second report, and none of them met
     assert lines[3] == [5, 0]
+
+
+def test_a_drained_ring_has_every_release(lines):
+    assert lines[4] == [0, 0]                # none outstanding, and no wait for one that never comes

@@ -185,6 +185,8 @@ k_gemm_fp8(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CU
           }
         }
       }
+      drain_ring(T::kStages, stage, wait_parity,
+                 [&](uint32_t s, uint32_t parity) { mbar_wait_inline(empty_bar(s), parity, ctl, kCodeProducer); });
     } else if (warp == 1) {
       // ------------------------------------------------------------ MMA issuer
       // The whole warp walks the loop and one lane issues: descriptors and addresses then live in
@@ -505,6 +507,8 @@ k_gemm_fp8_few(const __grid_constant__ CUtensorMap tma_w, const __grid_constant_
         wait_parity ^= 1u;
       }
     }
+    drain_ring(T::kStages, stage, wait_parity,
+               [&](uint32_t s, uint32_t parity) { mbar_wait_inline(empty_bar(s), parity, ctl, kCodeProducer); });
   } else if (warp == 1) {
     constexpr uint32_t idesc = make_idesc_e4m3(kTileRows, kBT);
     const uint64_t wdesc0 = make_kmajor_sw128_desc(base);

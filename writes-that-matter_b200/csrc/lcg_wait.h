@@ -32,4 +32,18 @@ LCG_HOST_DEVICE bool bounded_wait(volatile uint32_t* abort_flag, uint64_t limit_
   return true;
 }
 
+// The end of a ring's producer, which stands at (stage, parity) behind its last fill and would wait there for the
+// stage's release before the next: waits for the release of all stages.  They arrive in this CTA's barriers by
+// themselves, so it must not end before the last has.  A stage never filled is not waited for.
+template <class Wait>
+LCG_HOST_DEVICE void drain_ring(uint32_t stages, uint32_t stage, uint32_t parity, Wait wait) {
+  for (uint32_t i = 0; i < stages; ++i) {
+    wait(stage, parity);
+    if (++stage == stages) {
+      stage = 0;
+      parity ^= 1u;
+    }
+  }
+}
+
 }  // namespace lcg
