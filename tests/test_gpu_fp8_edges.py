@@ -1,0 +1,69 @@
+"""The 8-bit operators at the ends of what their documentation allows: padding beside NaN, gates whose exponential
+leaves fp32's range, empty batches, another current device."""
+import pytest
+import torch
+
+from gpu_util import seeded
+
+pytestmark = pytest.mark.gpu
+
+
+def test_another_current_device(monkeypatch):
+    """Every operator sets its tensors' device and calls itself when another one is current: the first question after
+    the current device is answered with one that is not the tensors'."""
+    from lcgemm import ops
+
+    x, nw = seeded((5, 256), 1), seeded((256,), 3, 0.1)
+    w, ws = ops.quantize_fp8(seeded((64, 256), 2), block_rows=128)
+    q, s = ops.quantize_fp8(x)
+    ids = torch.arange(5, device="cuda")
+    residual, out = x.clone(), torch.empty((5, 64), dtype=torch.bfloat16, device="cuda")
+    calls = (lambda: ops.quantize_fp8(x), lambda: ops.quantize_fp8(x, 128), lambda: ops.swiglu_fp8(x),
+             lambda: ops.add_rmsnorm_fp8(x, residual, nw, 1e-6), lambda: ops.add_rmsnorm_fp8(None, residual, nw, 1e-6),
+             lambda: (ops.gemm_fp8(q, s, w, ws),), lambda: (ops.gemm_fp8(q, s, w, ws, out),),
+             lambda: ops.token_logprobs(x, ids, 4))
+    real = ops._current_device
+    for call in calls:
+        want = [t.clone() for t in call()]
+        asked = []
+
+        def other():
+            asked.append(None)
+            return real() + 1 if len(asked) == 1 else real()
+
+        monkeypatch.setattr(ops, "_current_device", other)
+        got = call()
+        monkeypatch.setattr(ops, "_current_device", real)
+        assert len(asked) == 2 and torch.cuda.current_device() == 0
+        assert all(torch.equal(a.float(), b.float()) for a, b in zip(got, want))
+
+
+def test_the_norm_repeats_itself():
+    """A long prefill's norm: the same bits every time, and codes that are off from 64 bits only where the scaled
+    value lies within fp32's error of a border between two codes."""
+    from lcgemm import ops
+
+    m, k = 8192, 5120
+    g = torch.Generator(device="cuda").manual_seed(7)
+    spread = torch.exp(0.5 * torch.randn(k, generator=g, device="cuda"))
+    delta = (torch.randn((m, k), generator=g, device="cuda") * spread).to(torch.bfloat16)
+    residual = (3.0 * torch.randn((m, k), generator=g, device="cuda") * spread).to(torch.bfloat16)
+    w = (0.1 * torch.randn(k, generator=g, device="cuda")).to(torch.bfloat16)
+    q, s, h = ops.add_rmsnorm_fp8(delta, residual, w, 1e-6)
+    for _ in range(20):
+        again = ops.add_rmsnorm_fp8(delta, residual, w, 1e-6)
+        assert torch.equal(again[0].view(torch.uint8), q.view(torch.uint8))
+        assert torch.equal(again[1], s) and torch.equal(again[2], h)
+    assert torch.equal(h, (delta.float() + residual.float()).to(torch.bfloat16))
+    # err as in test_add_rmsnorm_fp8: its derivation holds for this K
+    err = (24 + 10) * 2.0 ** -25 + 8 * 2.0 ** -24
+    for i in range(0, m, 1024):
+        hd = h[i:i + 1024].double()
+        y = hd * torch.rsqrt((hd * hd).mean(-1, keepdim=True) + 1e-6) * (w.double() + 1.0)
+        blocks = y.view(1024, k // 128, 128)
+        scale = blocks.abs().amax(-1, keepdim=True) / 448.0
+        scaled = (blocks / scale).view(1024, k)
+        low, high = ((scaled * (1 + e)).clamp(-448.0, 448.0).float().to(torch.float8_e4m3fn).float() for e in (-2 * err, 2 * err))
+        got = q[i:i + 1024].float()
+        assert bool(((got == low) | (got == high)).all())
+        assert float((low != high).float().mean()) < 1e-3       # so nearly every code has one right value
