@@ -8,6 +8,41 @@ from gpu_util import seeded
 pytestmark = pytest.mark.gpu
 
 
+def padding(q):
+    m, k = q.shape
+    return torch.as_strided(q.view(torch.uint8), (m, q.stride(0) - k), (q.stride(0), 1), q.storage_offset() + k)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("k", [1, 8, 120, 129, 301, 1001])
+@pytest.mark.parametrize("rows", [1, 128])
+def test_padding_is_zero_beside_bad_values(rows, k, bad):
+    from lcgemm import ops
+
+    x = seeded((5, k), k)
+    x[2, k - 1] = bad
+    q, s = ops.quantize_fp8(x, block_rows=rows)
+    assert q.stride(0) % 16 == 0 and q.stride(0) > k and not bool(padding(q).any())
+    got = q.float() * s.repeat_interleave(rows, 0)[:5].repeat_interleave(128, 1)[:, :k]
+    last = k - 1 - (k - 1) % 128
+    assert bool(got[2, last:].isnan().all()) and not bool(got[:, :last].isnan().any())
+    # the codes of a block with a NaN are NaN by the definition, x * (448 / NaN)
+    assert bad == bad or bool(q[2, last:].float().isnan().all())
+
+
+@pytest.mark.parametrize("inter", [8, 136, 1000])
+def test_swiglu_padding_is_zero_beside_bad_values(inter):
+    from lcgemm import ops
+
+    z = seeded((4, 2 * inter), inter)
+    z[1, inter - 1], z[3, 2 * inter - 1] = float("nan"), float("inf")
+    q, s = ops.swiglu_fp8(z)
+    assert q.stride(0) > inter and not bool(padding(q).any())
+    got = q.float() * s.repeat_interleave(128, 1)[:, :inter]
+    last = inter - 1 - (inter - 1) % 128
+    assert bool(got[[1, 3], last:].isnan().all()) and not bool(got[[0, 2]].isnan().any())
+
+
 def test_another_current_device(monkeypatch):
     """Every operator sets its tensors' device and calls itself when another one is current: the first question after
     the current device is answered with one that is not the tensors'."""
