@@ -43,6 +43,32 @@ def test_swiglu_padding_is_zero_beside_bad_values(inter):
     assert bool(got[[1, 3], last:].isnan().all()) and not bool(got[[0, 2]].isnan().any())
 
 
+def test_swiglu_of_far_gates_and_large_products():
+    """silu(g) * u where e^-g or silu(g) alone leaves fp32's normal range and the product does not."""
+    from lcgemm import ops
+
+    gates = torch.cat([-torch.arange(60.0, 200.0, 0.5), -torch.tensor([300.0, 1e4, 3e38]), torch.tensor([0.0, 1.0, 88.0, 1e4])])
+    ups = torch.tensor([1.0, -1e6, 1e10, 1e20, -1e30, 3e38])
+    g = gates.to(torch.bfloat16)[:, None].expand(-1, len(ups)).reshape(-1)
+    u = ups.to(torch.bfloat16)[None, :].expand(len(gates), -1).reshape(-1)
+    keep = (g.double() * torch.sigmoid(g.double()) * u.double()).abs() < 3e38
+    g, u = g[keep], u[keep]
+    # a value to a row, so that each has a block and a scale of its own; seven small ones beside it
+    m = g.shape[0]
+    z = torch.zeros((m, 16), dtype=torch.bfloat16)
+    z[:, 0], z[:, 8] = g, u
+    z[:, 1:8] = -90.0
+    q, s = ops.swiglu_fp8(z.cuda())
+    y = z[:, :8].double() * torch.sigmoid(z[:, :8].double()) * z[:, 8:].double()
+    got = q.double().cpu() * s.double().cpu()
+    # The half exponential: its argument's rounding and constant 2^-18 each of at most 126 in base 2, its own 2^-22; it
+    # enters twice.  Four products, a sum, a reciprocal and the scaling: 2^-24 each, 2^-23 for the reciprocal.
+    err = 2 * (0.7 * (2.0 ** -18 + 2.0 ** -18) + 2.0 ** -22) + 8 * 2.0 ** -24
+    assert bool(((got - y).abs() <= (2.0 ** -4 + err) * y.abs() * 1.001 + s.double().cpu() * 2.0 ** -10).all())
+    want_s = y.abs().amax(1, keepdim=True).clamp_min(2.0 ** -100) / 448.0
+    assert bool(((s.double().cpu() - want_s).abs() <= (err + 2.0 ** -24) * want_s).all())
+
+
 def test_another_current_device(monkeypatch):
     """Every operator sets its tensors' device and calls itself when another one is current: the first question after
     the current device is answered with one that is not the tensors'."""
