@@ -459,7 +459,9 @@ def add(a: torch.Tensor, b: torch.Tensor, out: torch.Tensor | None = None) -> to
 # short: one allocation call per output, the raw stream handle, no context managers on the usual path.
 _current_device = torch.cuda.current_device
 _empty = torch.empty_strided
-_raw_stream = torch._C._cuda_getCurrentRawStream      # the handle, without the Python object around it
+# The handle, without the Python object around it; a build of torch without CUDA does not have it and gets no further
+# than the checks of the tensors.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 _F32 = torch.float32
 
 
