@@ -69,6 +69,14 @@ def test_swiglu_of_far_gates_and_large_products():
     assert bool(((s.double().cpu() - want_s).abs() <= (err + 2.0 ** -24) * want_s).all())
 
 
+def test_an_empty_batch_through_the_layer():
+    from lcgemm.layer import Fp8MlpLayer
+
+    layer = Fp8MlpLayer(4, seeded((256,), 3, 0.01), seeded((512, 256), 4, 0.02), seeded((256, 256), 5, 0.02))
+    for delta in (None, seeded((0, 256), 2)):
+        assert layer(seeded((0, 256), 1), delta).shape == (0, 256)
+
+
 def test_another_current_device(monkeypatch):
     """Every operator sets its tensors' device and calls itself when another one is current: the first question after
     the current device is answered with one that is not the tensors'."""

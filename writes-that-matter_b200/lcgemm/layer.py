@@ -141,7 +141,8 @@ class Fp8MlpLayer:
 
     def forward(self, x, delta=None):
         d, h = self.chain(delta, x)
-        return ops.add(h, d, out=self.out[:x.shape[0]])
+        out = self.out[:x.shape[0]]
+        return ops.add(h, d, out=out) if x.shape[0] > 0 else out
 
     __call__ = forward
     launches_per_forward = 5
