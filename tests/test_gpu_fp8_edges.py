@@ -77,6 +77,16 @@ def test_an_empty_batch_through_the_layer():
         assert layer(seeded((0, 256), 1), delta).shape == (0, 256)
 
 
+def test_a_prompt_on_the_host():
+    from lcgemm.model import DecoderConfig, RandomInitDecoder
+
+    model = RandomInitDecoder(DecoderConfig(layers=1, hidden=256, q_heads=4, kv_heads=2, head_dim=64, inter=256, vocab=999, seed=1))
+    tokens = torch.randint(0, 999, (40,), generator=torch.Generator().manual_seed(2))
+    want = model.prompt_logprobs(tokens.cuda(), top=3)
+    got = model.prompt_logprobs(tokens, top=3)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_another_current_device(monkeypatch):
     """Every operator sets its tensors' device and calls itself when another one is current: the first question after
     the current device is answered with one that is not the tensors'."""

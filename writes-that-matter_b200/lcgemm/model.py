@@ -206,6 +206,7 @@ class RandomInitDecoder:
             raise ValueError(f"a prompt of at least two tokens, got {tuple(token_ids.shape)}")
         if rows < 1:
             raise ValueError(f"rows must be positive, got {rows}")
+        token_ids = token_ids.to(self.device)           # a prefill takes ids from the host too
         final = self.prefill(token_ids, arm=arm)[1][:-1]
         parts = [ops.token_logprobs(F.linear(final[i:i + rows], self.lm_head), token_ids[1 + i:1 + i + rows], top=top)
                  for i in range(0, final.shape[0], rows)]
