@@ -432,7 +432,7 @@ struct FewParams {
   Scales a, b;
   __nv_bfloat16* c;
   int64_t ldc;
-  int32_t m, n, k_blocks, token_tiles, split;
+  int32_t m, n, k_blocks, split;      // m <= kBT: one tile of tokens
   int32_t* status;
 };
 
@@ -460,12 +460,9 @@ k_gemm_fp8_few(const __grid_constant__ CUtensorMap tma_w, const __grid_constant_
   const int lane = threadIdx.x & 31;
   const int rank = p.split > 1 ? static_cast<int>(cluster_ctarank()) : 0;
   const int tile = blockIdx.x / p.split;
-  const int tn = tile / p.token_tiles;
-  const int n0 = tn * kTileRows;
-  const int m0 = (tile - tn * p.token_tiles) * kBT;
+  const int n0 = tile * kTileRows;
   const int kb0 = static_cast<int>(static_cast<int64_t>(p.k_blocks) * rank / p.split);
   const int kb1 = static_cast<int>(static_cast<int64_t>(p.k_blocks) * (rank + 1) / p.split);
-  const int tokens = min(kBT, p.m - m0);
   const WaitCtl ctl{&misc_gen[1], p.status};
 
   if (threadIdx.x == 0) {
@@ -499,7 +496,7 @@ k_gemm_fp8_few(const __grid_constant__ CUtensorMap tma_w, const __grid_constant_
         mbar_arrive_expect_tx(full_bar(stage), T::kStageBytes);
         const uint32_t sw = base + stage * T::kStageBytes;
         tma_load_2d(sw, &tma_w, full_bar(stage), kb * kBlock, n0);
-        tma_load_2d(sw + kOperandBytes, &tma_x, full_bar(stage), kb * kBlock, m0);
+        tma_load_2d(sw + kOperandBytes, &tma_x, full_bar(stage), kb * kBlock, 0);
       }
       __syncwarp();
       if (++stage == T::kStages) {
@@ -547,14 +544,14 @@ k_gemm_fp8_few(const __grid_constant__ CUtensorMap tma_w, const __grid_constant_
     // Scales of kAhead blocks at a time, a's times b's, staged by all the read-back warps: [block][token].
     constexpr int kPer = (T::kAhead * kBT + kReadThreads - 1) / kReadThreads;
     float na[kPer], nb[kPer];
-    const float* sb = p.b.p + tn * p.b.row;
+    const float* sb = p.b.p + tile * p.b.row;
     auto fetch = [&](int kbs) {
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
         const int e = pt + i * kReadThreads;
         const int kb = kbs + e / kBT, j = e % kBT;
-        const bool in = e < T::kAhead * kBT && kb < kb1 && j < tokens;
-        na[i] = in ? __ldg(p.a.p + (m0 + j) * p.a.row + kb * p.a.blk) : 0.f;
+        const bool in = e < T::kAhead * kBT && kb < kb1 && j < p.m;
+        na[i] = in ? __ldg(p.a.p + j * p.a.row + kb * p.a.blk) : 0.f;
         nb[i] = in ? __ldg(sb + kb * p.b.blk) : 0.f;
       }
     };
@@ -621,9 +618,9 @@ k_gemm_fp8_few(const __grid_constant__ CUtensorMap tma_w, const __grid_constant_
         for (int j = 0; j < T::kCols / 2; ++j) {
           float lo, hi;
           unpack_f32x2(acc[j], lo, hi);
-          __nv_bfloat16* dst = p.c + static_cast<int64_t>(m0 + tok0 + 2 * j) * p.ldc + n0 + row;
-          if (tok0 + 2 * j < tokens) dst[0] = __float2bfloat16_rn(lo);
-          if (tok0 + 2 * j + 1 < tokens) dst[p.ldc] = __float2bfloat16_rn(hi);
+          __nv_bfloat16* dst = p.c + static_cast<int64_t>(tok0 + 2 * j) * p.ldc + n0 + row;
+          if (tok0 + 2 * j < p.m) dst[0] = __float2bfloat16_rn(lo);
+          if (tok0 + 2 * j + 1 < p.m) dst[p.ldc] = __float2bfloat16_rn(hi);
         }
       }
     } else {
@@ -648,7 +645,7 @@ k_gemm_fp8_few(const __grid_constant__ CUtensorMap tma_w, const __grid_constant_
     const int half = threadIdx.x >> 7;
     constexpr int kHalves = T::kThreads / kTileRows;
     if (half < kHalves && n0 + row < p.n) {
-      for (int j = rank + half * p.split; j < tokens; j += kHalves * p.split) {
+      for (int j = rank + half * p.split; j < p.m; j += kHalves * p.split) {
         const uint32_t addr = base + static_cast<uint32_t>(j * kTileRows + row) * 4u;
         float sum = 0.f;
         for (int r = 0; r < p.split; ++r) {
@@ -656,7 +653,7 @@ k_gemm_fp8_few(const __grid_constant__ CUtensorMap tma_w, const __grid_constant_
           asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(mapa_shared(addr, r)) : "memory");
           sum += v;
         }
-        p.c[static_cast<int64_t>(m0 + j) * p.ldc + n0 + row] = __float2bfloat16_rn(sum);
+        p.c[static_cast<int64_t>(j) * p.ldc + n0 + row] = __float2bfloat16_rn(sum);
       }
     }
     __syncwarp();
@@ -763,9 +760,8 @@ int run_few(const Call& q) {
   p.m = static_cast<int32_t>(q.m);
   p.n = static_cast<int32_t>(q.n);
   p.k_blocks = static_cast<int32_t>((q.k + kBlock - 1) / kBlock);
-  p.token_tiles = static_cast<int32_t>((q.m + kBT - 1) / kBT);
   p.status = q.status;
-  const int64_t tiles = static_cast<int64_t>(p.token_tiles) * ((q.n + kTileRows - 1) / kTileRows);
+  const int64_t tiles = (q.n + kTileRows - 1) / kTileRows;
   // Split K so that the GPU is filled: rounds of clusters times the K blocks of a CTA.  How many clusters of
   // a size run at once is asked once per device, for one CTA to an SM as the runtime counts them: the
   // GPU's parts are not multiples of each size (15 of 7, 22 of 6; 5120 x 17408 and one token, 40
@@ -804,7 +800,6 @@ int run_few(const Call& q) {
     }
   }
   p.split = split;
-  if (tiles * split > 0x7fffffffLL) return fail(LCG_ERR_UNSUPPORTED_SHAPE, "too many tiles");
   return launch(k_gemm_fp8_few<kBT>, static_cast<unsigned>(tiles * split), T::kThreads, T::kSmemBytes,
                 static_cast<unsigned>(split), q.stream, mw, mx, p);
 }
