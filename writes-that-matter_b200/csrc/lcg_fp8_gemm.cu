@@ -170,8 +170,8 @@ k_gemm_fp8(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CU
         const int a_row = tm * 2 * kTileRows + static_cast<int>(cta_rank) * kTileRows;
         const int b_row = tn * kBN + static_cast<int>(cta_rank) * T::kBRows;
         for (int kb = 0; kb < p.k_blocks; ++kb) {
-          const bool ok = mbar_wait_inline(empty_bar(stage), wait_parity, ctl, kCodeProducer);
-          if (elect_one() && ok) {
+          mbar_wait_inline(empty_bar(stage), wait_parity, ctl, kCodeProducer);
+          if (elect_one()) {
             if (leader) mbar_arrive_expect_tx(full_bar(stage), 2 * T::kStageBytes);
             const uint32_t sa = base + stage * T::kStageBytes;
             const uint32_t bar = full_leader + 8u * stage;
@@ -208,10 +208,10 @@ k_gemm_fp8(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CU
             const uint64_t soff = static_cast<uint64_t>(stage * (T::kStageBytes >> 4));
             bool acc_ok, full_ok;
             mbar_try_wait_both(acc_empty_bar(as), acc_parity, full_bar(stage), parity, acc_ok, full_ok);
-            if (!acc_ok) acc_ok = mbar_wait_inline(acc_empty_bar(as), acc_parity, ctl, kCodeMmaAcc);
-            if (!full_ok) full_ok = mbar_wait_inline(full_bar(stage), parity, ctl, kCodeMmaFull);
+            if (!acc_ok) mbar_wait_inline(acc_empty_bar(as), acc_parity, ctl, kCodeMmaAcc);
+            if (!full_ok) mbar_wait_inline(full_bar(stage), parity, ctl, kCodeMmaFull);
             tcgen05_fence_after();
-            if (elect_one() && acc_ok && full_ok) {
+            if (elect_one()) {
 #pragma unroll
               for (int k = 0; k < kBlock / kSliceK; ++k)
                 umma_fp8<2>(tmem_base + as * kBN, adesc0 + soff + 2u * k, bdesc0 + soff + 2u * k, idesc, k > 0);
@@ -226,8 +226,8 @@ k_gemm_fp8(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CU
             }
           }
           while (as != 0) {          // every tile starts at stage 0
-            const bool ok = mbar_wait_inline(acc_empty_bar(as), acc_parity, ctl, kCodeMmaAcc);
-            if (elect_one() && ok) umma_commit<2>(acc_full_bar(as));
+            mbar_wait_inline(acc_empty_bar(as), acc_parity, ctl, kCodeMmaAcc);
+            if (elect_one()) umma_commit<2>(acc_full_bar(as));
             __syncwarp();
             next_stage();
           }
@@ -491,8 +491,8 @@ k_gemm_fp8_few(const __grid_constant__ CUtensorMap tma_w, const __grid_constant_
   if (warp == 0) {
     uint32_t stage = 0, wait_parity = 1;
     for (int kb = kb0; kb < kb1; ++kb) {
-      const bool ok = mbar_wait_inline(empty_bar(stage), wait_parity, ctl, kCodeProducer);
-      if (elect_one() && ok) {
+      mbar_wait_inline(empty_bar(stage), wait_parity, ctl, kCodeProducer);
+      if (elect_one()) {
         mbar_arrive_expect_tx(full_bar(stage), T::kStageBytes);
         const uint32_t sw = base + stage * T::kStageBytes;
         tma_load_2d(sw, &tma_w, full_bar(stage), kb * kBlock, n0);
@@ -512,11 +512,11 @@ k_gemm_fp8_few(const __grid_constant__ CUtensorMap tma_w, const __grid_constant_
     const uint64_t xdesc0 = make_kmajor_sw128_desc(base + kOperandBytes);
     uint32_t stage = 0, parity = 0, as = 0, acc_parity = 1;
     for (int kb = kb0; kb < kb1; ++kb) {
-      bool ok = mbar_wait_inline(acc_empty_bar(as), acc_parity, ctl, kCodeMmaAcc);
-      ok &= mbar_wait_inline(full_bar(stage), parity, ctl, kCodeMmaFull);
+      mbar_wait_inline(acc_empty_bar(as), acc_parity, ctl, kCodeMmaAcc);
+      mbar_wait_inline(full_bar(stage), parity, ctl, kCodeMmaFull);
       tcgen05_fence_after();
       const uint64_t soff = static_cast<uint64_t>(stage * (T::kStageBytes >> 4));
-      if (elect_one() && ok) {
+      if (elect_one()) {
 #pragma unroll
         for (int k = 0; k < kBlock / kSliceK; ++k)
           umma_fp8<1>(tmem_base + as * kBT, wdesc0 + soff + 2u * k, xdesc0 + soff + 2u * k, idesc, k > 0);

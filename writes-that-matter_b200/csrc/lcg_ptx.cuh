@@ -154,11 +154,10 @@ __device__ __forceinline__ void mbar_wait(uint32_t bar, uint32_t parity, const W
 }
 
 // The same without a call: for warps whose registers are full of accumulators, which a call's
-// register convention would move about.  Whether the wait was met.
-__device__ __forceinline__ bool mbar_wait_inline(uint32_t bar, uint32_t parity, const WaitCtl& ctl, int code) {
-  return bounded_wait(ctl.abort_flag, ctl.limit_ns, [&] { return mbar_try_wait(bar, parity); },
-                      [] { return globaltimer_ns(); },
-                      [&] { if (ctl.status != nullptr) atomicCAS(ctl.status, 0, code); });
+// register convention would move about.
+__device__ __forceinline__ void mbar_wait_inline(uint32_t bar, uint32_t parity, const WaitCtl& ctl, int code) {
+  bounded_wait(ctl.abort_flag, ctl.limit_ns, [&] { return mbar_try_wait(bar, parity); }, [] { return globaltimer_ns(); },
+               [&] { if (ctl.status != nullptr) atomicCAS(ctl.status, 0, code); });
 }
 
 // Bounded wait on a monotonically increasing shared-memory counter.

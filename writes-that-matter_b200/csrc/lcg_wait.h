@@ -11,25 +11,23 @@
 namespace lcg {
 
 // Tries until `try_wait` (which may suspend the thread for a while) is met, `abort_flag` is set, or `limit_ns` of
-// `now` have passed: then the flag is set and `give_up` called.  Whether the wait was met: what it was for is issued
-// only then, so that once a wait has run out no copies or products pile up behind it.
+// `now` have passed: then the flag is set and `give_up` called.
 template <class TryWait, class Now, class GiveUp>
-LCG_HOST_DEVICE bool bounded_wait(volatile uint32_t* abort_flag, uint64_t limit_ns, TryWait try_wait, Now now,
+LCG_HOST_DEVICE void bounded_wait(volatile uint32_t* abort_flag, uint64_t limit_ns, TryWait try_wait, Now now,
                                   GiveUp give_up) {
   uint64_t t0 = 0;
   // the timer is read once in 64 tries: reading it takes longer than most waits
   for (uint32_t tries = 1; !try_wait(); ++tries) {
-    if (*abort_flag) return false;
+    if (*abort_flag) return;
     if ((tries & 63u) != 0) continue;
     const uint64_t t = now();
     if (t0 == 0) t0 = t;
     if (t - t0 > limit_ns) {
       *abort_flag = 1u;
       give_up();
-      return false;
+      return;
     }
   }
-  return true;
 }
 
 // The end of a ring's producer, which stands at (stage, parity) behind its last fill and would wait there for the
