@@ -350,11 +350,12 @@ int lcg_add(const void* a, const void* b, void* out, int64_t n, void* stream);
  * A producer scales one block by a = max(max |x|, 2^-100): scale = a / 448, code =
  * e4m3(x * (448 / a)), with correctly rounded fp32 arithmetic and one rounding to e4m3 (nearest
  * even, saturating).  A block that holds an infinity or a NaN decodes to NaN throughout.  The columns
- * from K to the next multiple of 16 receive zero codes. */
+ * from K to the next multiple of 16 receive zero codes, beside a NaN too. */
 
 /* Codes and scales of a bf16 matrix x (M, K) with leading dimension ldx.  block_rows = 1: a scale
- * per row and block (activations); 128: a scale per 128 x 128 tile (weights).  Any M, K >= 1; rows
- * that are not 16-byte aligned are read value by value. */
+ * per row and block (activations); 128: a scale per 128 x 128 tile (weights).  K from 1 to
+ * 2^31 - 256, M from 1 to 2^30 / ceil(K / 128) rows, or 65535 rows of tiles; rows may not overlap (ldx >= K), and
+ * those that are not 16-byte aligned are read value by value. */
 int lcg_quantize_fp8(const void* x, int64_t M, int64_t K, int64_t ldx, int block_rows, void* q,
                      int64_t ldq, float* scale, int64_t scale_row_stride,
                      int64_t scale_block_stride, void* stream);
@@ -362,28 +363,33 @@ int lcg_quantize_fp8(const void* x, int64_t M, int64_t K, int64_t ldx, int block
 /* lcg_add_rmsnorm with an 8-bit result: h = bf16(delta + residual) -> residual_out (may alias
  * residual), y = h * rsqrt(mean(h^2) + eps) * (norm_weight + 1), quantised by rows from its fp32
  * value (it is never rounded to bf16).  delta may be NULL: h is the residual, residual_out is
- * neither needed nor written.  Contiguous (M, K), K % 8 == 0, K <= 24576. */
+ * neither needed nor written.  Contiguous (M, K), M < 2^31, K % 8 == 0, K <= 24576. */
 int lcg_add_rmsnorm_fp8(const void* delta, const void* residual, const void* norm_weight,
                         int64_t M, int64_t K, float eps, void* residual_out, void* q, int64_t ldq,
                         float* scale, int64_t scale_row_stride, int64_t scale_block_stride,
                         void* stream);
 
-/* lcg_swiglu with an 8-bit result: silu(gate) * up quantised by rows from its fp32 value.  z is
- * (M, 2*I) with ldz; I % 8 == 0. */
+/* lcg_swiglu with an 8-bit result: silu(gate) * up quantised by rows from its fp32 value, which is right
+ * also where silu(gate) alone is below fp32's range.  z is (M, 2*I) with ldz; I % 8 == 0, I <= 2^30 - 256,
+ * M * ceil(I / 128) <= 2^30. */
 int lcg_swiglu_fp8(const void* z, int64_t M, int64_t I, int64_t ldz, void* q, int64_t ldq,
                    float* scale, int64_t scale_row_stride, int64_t scale_block_stride,
                    void* stream);
 
 /* C = bf16(sum over blocks t of a_scale[m, t] * b_scale[n / 128, t] * (a . b over block t)), block
  * sums and scaled sum in fp32.  a (M, K) and b (N, K) codes, scales of `block_rows` 1 and 128; c
- * (M, N) bf16, 16-byte aligned, ldc % 8 == 0.  Any M, N, K >= 1, one token included. */
+ * (M, N) bf16, 16-byte aligned, ldc % 8 == 0.  M, N and K from 1 (one token included) to 2^30, at most
+ * 2^31 - 1 tiles of 256 x 128.  A block's two scales are multiplied first, in fp32: a product outside
+ * [2^-126, 2^128) loses bits or is 0 below and turns the block's part into an infinity, or NaN where its sum
+ * is 0, above.  (Operands of ordinary size are far from both: the product of the scales of blocks whose largest values
+ * are x and y is x * y / 200704.) */
 int lcg_gemm_fp8(const void* a, int64_t lda, const float* a_scale, int64_t a_scale_row_stride,
                  int64_t a_scale_block_stride, const void* b, int64_t ldb, const float* b_scale,
                  int64_t b_scale_row_stride, int64_t b_scale_block_stride, void* c, int64_t ldc,
                  int64_t M, int64_t N, int64_t K, int32_t* status, void* stream);
 
 /* ---- log probabilities ----------------------------------------------------
- * For each row of logits (M, V), V <= 2^20, leading dimension ld, of type bf16, fp16 or fp32:
+ * For each row of logits (M, V), M < 2^28, V <= 2^20, leading dimension ld, of type bf16, fp16 or fp32:
  *   logprob = x[token] - ln(sum e^x)       entropy = -sum p ln p
  * and the `top` (0..32, at most V) largest values with their log probabilities, largest first,
  * equal values by rising id.  tokens: M ids of token_bytes (4 or 8) bytes each.  A masked value

@@ -146,3 +146,18 @@ def test_the_norm_repeats_itself():
         got = q[i:i + 1024].float()
         assert bool(((got == low) | (got == high)).all())
         assert float((low != high).float().mean()) < 1e-3       # so nearly every code has one right value
+
+
+@pytest.mark.parametrize("m", [3, 300])
+def test_scale_products_at_the_ends_of_their_range(m):
+    """The product of a block's two scales may be anything in fp32's normal range, the scales themselves too."""
+    from lcgemm import ops
+
+    n, k = 260, 384
+    g = torch.Generator(device="cuda").manual_seed(5)
+    a = torch.randint(-1, 2, (m, k), generator=g, device="cuda").to(torch.float8_e4m3fn)
+    b = torch.randint(-1, 2, (n, k), generator=g, device="cuda").to(torch.float8_e4m3fn)
+    for low, high in ((-63, -63), (-126, 0), (7, -126), (63, 55), (127, -9), (-9, 127)):
+        sa, sb = torch.full((m, 3), 2.0 ** low, device="cuda"), torch.full((3, 3), 2.0 ** high, device="cuda")
+        want = ((a.double() @ b.double().t()) * 2.0 ** (low + high)).to(torch.bfloat16)
+        assert torch.equal(ops.gemm_fp8(a, sa, b, sb), want)

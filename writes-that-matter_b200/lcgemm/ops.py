@@ -588,7 +588,8 @@ def gemm_fp8(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: t
     """``a @ b.T`` in bf16 from e4m3 codes ``a (M, K)`` and ``b (N, K)`` with one fp32 scale per block of
     128: ``a_scale (M, ceil(K / 128))``, ``b_scale (ceil(N / 128), ceil(K / 128))``, of any strides (the
     quantisers' are the fastest).  Codes have unit stride along K and a row pitch of a multiple of 16
-    bytes, as the quantisers return them.  Each block's sum and the scaled sum are fp32."""
+    bytes, as the quantisers return them.  Each block's sum and the scaled sum are fp32; a block's two scales are
+    multiplied first, so their product has to lie in fp32's normal range too (``include/lcgemm_b200.h``)."""
     for t, what in ((a, "a"), (b, "b"), (a_scale, "a_scale"), (b_scale, "b_scale")):
         _need_cuda(t, what)
         if t.dim() != 2:
