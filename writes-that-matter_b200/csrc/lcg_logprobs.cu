@@ -16,10 +16,10 @@
 // holds.  (The second rule for every row, with its threshold searched by the whole CTA, took longer than
 // the pass: 436 us against 199 for 4096 rows of 151936 bf16 without alternatives.)
 //
-// Many rows: 4096 x 151936 bf16 without alternatives run at HBM's rate (203 us, 190 at the copy rate; 66
-// instructions to a warp's 512 bytes, the exponential unit at 2/3 of its rate); 20 alternatives add
-// 9300 instructions a row, which no longer fit beside the pass (239 us).  One row is bound by the
-// latency of the selection.  A row is one CTA's, or a cluster's of up to eight when there
+// Many rows: 4096 x 151936 bf16 without alternatives run at HBM's rate (198 us of device time, up to 220
+// among other calls; 190 at the copy rate; 66 instructions to a warp's 512 bytes, the exponential unit at 2/3 of its
+// rate); 20 alternatives add 9300 instructions a row, which no longer fit beside the pass (238 and up to 270 us).  One
+// row is bound by the latency of the selection.  A row is one CTA's, or a cluster's of up to eight when there
 // are too few rows to fill the GPU; the CTAs' parts are joined through distributed shared memory in
 // rank order, so the result does not depend on timing.
 #include <cuda_bf16.h>
