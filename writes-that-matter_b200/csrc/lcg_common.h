@@ -29,6 +29,8 @@ void count_launch(int n = 1);
 int make_tensor_map(CUtensorMap* map, CUtensorMapDataType type, int elt_bytes, const void* base,
                     int64_t inner, int64_t outer, int64_t ld, int box_outer, const char* what);
 int sm_count();
+// Whether the address is a multiple of `bytes`, a power of two; NULL is one of all.
+inline bool aligned(const void* p, unsigned bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 // Tile rows kept open at once: the divisor-free version of "minimise a + groups / a".
 int pick_group_m(int tiles_m, int groups);
 

@@ -431,6 +431,7 @@ int check_codes(const void* q, int64_t ldq, int64_t K, const float* scale) {
     return fail(LCG_ERR_BAD_ARG, "the codes' pitch must be a multiple of 16 bytes and hold K=%lld rounded up to one, got %lld",
                 (long long)K, (long long)ldq);
   if (!aligned16(q)) return fail(LCG_ERR_MISALIGNED, "the codes must be 16-byte aligned");
+  if (!aligned(scale, 4)) return fail(LCG_ERR_MISALIGNED, "the scales must be aligned to their type");
   return LCG_OK;
 }
 
@@ -459,6 +460,7 @@ extern "C" int lcg_quantize_fp8(const void* x, int64_t M, int64_t K, int64_t ldx
   if (M < 1 || K < 1 || K > 0x7fffff00LL)
     return fail(LCG_ERR_UNSUPPORTED_SHAPE, "bad extents M=%lld K=%lld", (long long)M, (long long)K);
   if (ldx < K && M > 1) return fail(LCG_ERR_BAD_ARG, "leading dimension below extent");
+  if (!aligned(x, 2)) return fail(LCG_ERR_MISALIGNED, "x must be aligned to its type");
   if (int e = check_codes(q, ldq, K, scale)) return e;
   const bool vec = aligned16(x) && (ldx % 8 == 0 || M == 1);
   const int64_t kblocks = (K + kBlock - 1) / kBlock;

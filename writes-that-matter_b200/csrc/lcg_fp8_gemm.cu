@@ -827,6 +827,8 @@ extern "C" int lcg_gemm_fp8(const void* a, int64_t lda, const float* a_scale, in
     return fail(LCG_ERR_MISALIGNED, "codes must be 16-byte aligned with a pitch of a multiple of 16 bytes");
   if (ldc % 8 != 0 || (reinterpret_cast<uintptr_t>(c) & 15u) != 0)
     return fail(LCG_ERR_MISALIGNED, "the output must be 16-byte aligned with a pitch of a multiple of 8 elements");
+  if (!aligned(a_scale, 4) || !aligned(b_scale, 4) || !aligned(status, 4))
+    return fail(LCG_ERR_MISALIGNED, "scales and status must be aligned to their type");
   if (((M + 255) / 256) * ((N + 127) / 128) > 0x7fffffffLL) return fail(LCG_ERR_UNSUPPORTED_SHAPE, "too many tiles");
   const Call q{a, b, lda, ldb, Scales{a_scale, a_scale_row_stride, a_scale_block_stride},
                Scales{b_scale, b_scale_row_stride, b_scale_block_stride}, c, ldc, M, N, K, status,

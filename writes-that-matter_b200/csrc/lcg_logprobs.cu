@@ -709,9 +709,10 @@ extern "C" int lcg_token_logprobs(const void* logits, int dtype, int64_t M, int6
     return fail(LCG_ERR_BAD_ARG, "top must be between 0 and min(%d, V), got %d", kMaxTop, top);
   if (dtype != LCG_DTYPE_BF16 && dtype != LCG_DTYPE_FP16 && dtype != LCG_DTYPE_FP32)
     return fail(LCG_ERR_BAD_ARG, "unknown dtype %d", dtype);
-  const uintptr_t width = dtype == LCG_DTYPE_FP32 ? 4 : 2;
-  if (reinterpret_cast<uintptr_t>(logits) % width != 0)
-    return fail(LCG_ERR_MISALIGNED, "logits must be aligned to their type");
+  const unsigned width = dtype == LCG_DTYPE_FP32 ? 4 : 2;
+  if (!aligned(logits, width) || !aligned(tokens, token_bytes) || !aligned(logprob, 4) || !aligned(entropy, 4) ||
+      (top > 0 && (!aligned(top_logprobs, 4) || !aligned(top_ids, 8))))
+    return fail(LCG_ERR_MISALIGNED, "logits, tokens and results must be aligned to their types");
   Params p;
   p.logits = logits;
   p.tokens = tokens;
