@@ -161,3 +161,24 @@ def test_scale_products_at_the_ends_of_their_range(m):
         sa, sb = torch.full((m, 3), 2.0 ** low, device="cuda"), torch.full((3, 3), 2.0 ** high, device="cuda")
         want = ((a.double() @ b.double().t()) * 2.0 ** (low + high)).to(torch.bfloat16)
         assert torch.equal(ops.gemm_fp8(a, sa, b, sb), want)
+
+
+@pytest.mark.parametrize("m", [1, 70, 129, 300])
+@pytest.mark.parametrize("n", [1, 3, 7, 8, 9, 63, 64, 65, 127, 129])
+def test_narrow_products(m, n):
+    """Fewer columns than a 16-byte piece, and around the edges of a staged store; one K value to a block and a bit."""
+    from lcgemm import ops
+
+    g = torch.Generator(device="cuda").manual_seed(m + n)
+    for k in (1, 16, 31, 128, 129):
+        pitch = (k + 15) // 16 * 16
+        a, b = (torch.randint(-4, 5, (rows, pitch), generator=g, device="cuda").to(torch.float8_e4m3fn)[:, :k] for rows in (m, n))
+        sa = torch.exp2(torch.randint(-3, 1, (m, -(-k // 128)), generator=g, device="cuda").float())
+        sb = torch.exp2(torch.randint(-3, 1, (-(-n // 128), -(-k // 128)), generator=g, device="cuda").float())
+        wide_a = a.double() * sa.double().repeat_interleave(128, 1)[:, :k]
+        wide_b = b.double() * sb.double().repeat_interleave(128, 0)[:n].repeat_interleave(128, 1)[:, :k]
+        big = torch.full((m + 2, (n + 7) // 8 * 8 + 8), 7.0, dtype=torch.bfloat16, device="cuda")
+        out = ops.gemm_fp8(a, sa, b, sb, out=big[1:m + 1, :n])
+        assert torch.equal(out, (wide_a @ wide_b.t()).to(torch.bfloat16))
+        assert bool((big[0] == 7.0).all() and (big[m + 1] == 7.0).all() and (big[:, n:] == 7.0).all())
+    ops.check_status()
